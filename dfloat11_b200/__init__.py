@@ -10,13 +10,13 @@ from .dfloat11 import (DFloat11Model, TensorManager, check_status, compress_in_p
 from . import ops  # noqa: F401
 from .generation import GraphedGreedyDecoder
 from .ops import (aux_bytes, decode, decode_prepared, decode_range_prepared, decode_rows_prepared, gemv_prepared,
-                  prepare, seek_interval)
+                  kv_append, kv_attention, kv_read, prepare, sample, seek_interval)
 
 __all__ = [
     "DFloat11Model", "TensorManager", "compress_in_place", "compress_model", "get_hook", "get_no_split_classes",
     "load_and_replace_tensors", "check_status", "stats",
     "UnrepresentableError", "encode_weights", "get_codec", "get_luts", "split_bf16", "validate_unit",
     "aux_bytes", "decode", "decode_prepared", "decode_range_prepared", "decode_rows_prepared", "gemv_prepared",
-    "prepare", "seek_interval", "ops",
+    "prepare", "seek_interval", "ops", "kv_append", "kv_attention", "kv_read", "sample",
     "GraphedGreedyDecoder",
 ]

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int32, c_int64, c_uint32, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int32, c_int64, c_uint32, c_void_p
 
 from .build import LIB_PATH, _stale, build_lib
 
@@ -21,6 +21,11 @@ STATUS_BAD_TABLE = 1
 STATUS_BAD_POSITIONS = 2
 STATUS_TRUNCATED = 4
 STATUS_TIMEOUT = 8
+STATUS_EMPTY_ROW = 16
+
+TYPE_BF16, TYPE_FP16, TYPE_FP32 = 0, 1, 2
+KV_INT8, KV_E4M3 = 0, 1
+KV_MAX_HEAD_DIM = 256
 
 # every symbol declared in include/df11.h: name -> (restype, argtypes)
 SIGNATURES = {
@@ -60,6 +65,16 @@ SIGNATURES = {
                                           c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int32, c_void_p]),
     "df11_encode_host": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_uint32, c_void_p, c_int64,
                                    c_void_p, c_int64, c_void_p, c_int64, c_int32]),
+    "df11_kv_append": (c_int32, [c_void_p] * 2 + [c_int64] * 6 + [c_void_p] * 5 + [c_int64, c_int64, c_int32, c_int64,
+                                 c_int32, c_int64, c_int32, c_int32, c_void_p, c_int32, c_void_p]),
+    "df11_kv_read": (c_int32, [c_void_p] * 6 + [c_int64, c_int32, c_int64, c_int32, c_int64, c_int64, c_int32, c_int32,
+                               c_int32, c_void_p]),
+    "df11_kv_attention_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int64, c_int32, c_int64, c_int32]),
+    "df11_kv_attention": (c_int32, [c_void_p] + [c_int64] * 3 + [c_void_p] * 5 + [c_int64, c_void_p, c_int64, c_void_p,
+                                    c_void_p, c_int64, c_int64, c_int32, c_int32, c_int64, c_int32, c_int64, c_int32,
+                                    c_float, c_int32, c_int32, c_int32, c_void_p]),
+    "df11_sample": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int64, c_void_p, c_void_p, c_double, c_void_p,
+                              c_int32, c_void_p, c_double, c_void_p, c_double, c_void_p, c_void_p, c_int32, c_void_p]),
 }
 
 

@@ -14,8 +14,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libdf11.so")
-SOURCES = ["df11_decode.cu", "df11_encode.cu", "df11_allreduce.cu", "df11_host.cpp"]
-HEADERS = ["df11_common.h", "df11_error.h", os.path.join("..", "..", "include", "df11.h")]
+SOURCES = ["df11_decode.cu", "df11_encode.cu", "df11_allreduce.cu", "df11_kv.cu", "df11_sample.cu",
+           "df11_host.cpp"]
+HEADERS = ["df11_common.h", "df11_error.h", "df11_launch.h", os.path.join("..", "..", "include", "df11.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,4 +1,4 @@
-"""Torch-facing launchers of the libdf11 decode entry points.
+"""Torch-facing launchers of the libdf11 entry points.
 
 These stand where the reference calls its cupy kernel object
 (``_decode(grid=..., block=..., shared_mem=..., args=[...])``, dfloat11/dfloat11.py:142-151
@@ -215,4 +215,192 @@ def gemv_prepared(luts: torch.Tensor, encoded_exponent: torch.Tensor, sign_manti
         out.data_ptr(), bias.data_ptr() if bias is not None else None, partials.data_ptr(),
         int(first_element), int(n_rows), int(in_features), int(m), luts.shape[0], encoded_exponent.numel(),
         sign_mantissa.numel(), status.data_ptr() if status is not None else None, device.index, _stream(device)))
+    return out
+
+
+# ------------------------------------------------------------------ operators of a generation step
+_ELEMENT_TYPES = {torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16, torch.float32: _lib.TYPE_FP32}
+KV_FORMATS = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_E4M3}
+
+
+def _activation(name: str, t: torch.Tensor, shape, device: Optional[torch.device]) -> torch.device:
+    """Checks of a ``[batch, heads, tokens, head_dim]`` activation: on ``device``, BF16 or FP16, no gradient
+    asked for, any strides as long as the last dimension is contiguous."""
+    if not t.is_cuda:
+        raise RuntimeError(f"df11 kernels need CUDA tensors; `{name}` is on {t.device}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"`{name}` is on {t.device}, expected {device}")
+    if t.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"`{name}` must be bfloat16 or float16, not {t.dtype}")
+    if t.dim() != 4 or (shape is not None and any(want is not None and have != want for have, want in zip(t.shape, shape))):
+        raise RuntimeError(f"`{name}` has shape {tuple(t.shape)}, expected {shape or '[batch, heads, tokens, head_dim]'}")
+    if t.numel() and t.stride(3) != 1:
+        raise RuntimeError(f"the last dimension of `{name}` must be contiguous")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"`{name}` requires a gradient, which this inference operator does not have; "
+                           "call it under torch.no_grad()")
+    return t.device
+
+
+def _cache(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor):
+    """Checks of the four tensors of a quantised cache; returns (device, format, batch, heads, slots, head_dim)."""
+    device = _require_cuda(k_codes=k_codes, k_scales=k_scales, v_codes=v_codes, v_scales=v_scales)
+    if k_codes.dtype not in KV_FORMATS or v_codes.dtype != k_codes.dtype:
+        raise RuntimeError("`k_codes` and `v_codes` must both be int8 or both be float8_e4m3fn")
+    if k_codes.dim() != 4 or v_codes.shape != k_codes.shape:
+        raise RuntimeError("`k_codes` and `v_codes` must be [batch, kv_heads, max_slots, head_dim], of one shape")
+    for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if t.dtype != torch.float32 or t.shape != k_codes.shape[:3]:
+            raise RuntimeError(f"`{name}` must be float32 [batch, kv_heads, max_slots]")
+    return (device, KV_FORMATS[k_codes.dtype], *k_codes.shape)
+
+
+def _per_sequence(name: str, t: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
+    _require_cuda(**{name: t})
+    if t.device != device:
+        raise RuntimeError(f"`{name}` is on {t.device}, expected {device}")
+    if t.dtype != torch.int64 or t.numel() not in (1, batch):
+        raise RuntimeError(f"`{name}` must be an int64 tensor of 1 or {batch} elements")
+    return t
+
+
+def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+              v_scales: torch.Tensor, positions: torch.Tensor, status: Optional[torch.Tensor] = None) -> None:
+    """Quantises new keys and values into the cache: token ``i`` of sequence ``b`` goes to slot ``positions[b] + i``.
+
+    ``k``, ``v``: ``[batch, kv_heads, tokens, head_dim]`` BF16 or FP16, any strides as long as the last dimension is
+    contiguous.  ``k_codes``, ``v_codes``: ``[batch, kv_heads, max_slots, head_dim]`` int8 or float8_e4m3fn -- the
+    dtype is the format --, ``k_scales``, ``v_scales``: float32 ``[batch, kv_heads, max_slots]``; ``head_dim`` is a
+    multiple of 16, at most 256.  A row ``x`` of largest magnitude ``a`` gets ``scale = a / 127`` (e4m3: ``a / 448``)
+    and stands for ``code * scale``, with the code nearest to ``x / scale`` (ties to even); a row with an infinity or
+    a NaN stands for NaNs.  ``positions``: int64, one per sequence or one for all.  Tokens whose slot the cache does not
+    have are left out and set ``STATUS_BAD_POSITIONS`` in ``status``."""
+    device, fmt, batch, heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+    _activation("k", k, (batch, heads, None, dim), device)
+    _activation("v", v, (batch, heads, k.shape[2], dim), device)
+    if v.dtype != k.dtype:
+        raise RuntimeError("`k` and `v` must have one dtype")
+    _per_sequence("positions", positions, batch, device)
+    _require_cuda(k_codes=k_codes, status=status)
+    if not k.numel():
+        return
+    _lib.check(_lib.lib.df11_kv_append(
+        k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k_codes.data_ptr(), k_scales.data_ptr(),
+        v_codes.data_ptr(), v_scales.data_ptr(), positions.data_ptr(), positions.numel(), batch, heads, k.shape[2], dim,
+        slots, _ELEMENT_TYPES[k.dtype], fmt, status.data_ptr() if status is not None else None, device.index,
+        _stream(device)))
+
+
+def kv_read(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, first_slot: int,
+            n_slots: int, dtype: torch.dtype = torch.bfloat16, out=None):
+    """Slots ``[first_slot, first_slot + n_slots)`` of every sequence as ``(k, v)``, each
+    ``[batch, kv_heads, n_slots, head_dim]`` in ``dtype`` (BF16 or FP16): ``code * scale`` in fp32, rounded once.
+    ``out`` may hold the two contiguous tensors to fill."""
+    device, fmt, batch, heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+    if dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError(f"`dtype` must be bfloat16 or float16, not {dtype}")
+    first_slot, n_slots = int(first_slot), int(n_slots)
+    if first_slot < 0 or n_slots < 0 or first_slot + n_slots > slots:
+        raise RuntimeError(f"slots {first_slot} .. {first_slot + n_slots} are not in a cache of {slots}")
+    shape = (batch, heads, n_slots, dim)
+    if out is None:
+        k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+    else:
+        k, v = out
+        _require_cuda(k_codes=k_codes, k=k, v=v)
+        if any(t.dtype != dtype or tuple(t.shape) != shape for t in (k, v)):
+            raise RuntimeError(f"`out` must be two {dtype} tensors of shape {shape}")
+    if k.numel():
+        _lib.check(_lib.lib.df11_kv_read(
+            k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), k.data_ptr(), v.data_ptr(),
+            batch, heads, slots, dim, first_slot, n_slots, _ELEMENT_TYPES[dtype], fmt, device.index, _stream(device)))
+    return k, v
+
+
+def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
+                 v_scales: torch.Tensor, lengths: torch.Tensor, first: Optional[torch.Tensor] = None,
+                 scale: Optional[float] = None, window: int = 0, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a few new tokens over a quantised cache, which is read in its 8-bit form.
+
+    ``q``: ``[batch, heads, queries, head_dim]`` BF16 or FP16, any strides as long as the last dimension is contiguous;
+    head ``h`` reads the keys of head ``h // (heads // kv_heads)``.  The cache is described at ``kv_append``.
+    ``lengths``: int64, one per sequence or one for all: the filled slots, the new tokens' included, so that query ``i``
+    stands at ``p = length - queries + i`` and sees slots ``max(first, p - window + 1) .. p`` (``window`` 0: from
+    ``first``, which is 0 when it is not given; left padding lies before it).  ``scale`` defaults to
+    ``head_dim ** -0.5``.  The result is ``[batch, queries, heads, head_dim]`` in ``q``'s dtype, as the projection that
+    follows wants it; a query that sees nothing gives zeros.  Any number of queries works; what the kernel is made for
+    is one to some sixteen rows per key head (a long prompt is better read back with ``kv_read``).
+    Working memory is allocated per call, so calls may overlap on different streams."""
+    device, fmt, batch, kv_heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+    _activation("q", q, (batch, None, None, dim), device)
+    heads, queries = q.shape[1], q.shape[2]
+    if heads < 1 or heads % kv_heads:
+        raise RuntimeError(f"{heads} query heads on {kv_heads} key heads")
+    _per_sequence("lengths", lengths, batch, device)
+    if first is not None:
+        _per_sequence("first", first, batch, device)
+    if window < 0:
+        raise RuntimeError("`window` must not be negative")
+    if out is None:
+        out = torch.empty(batch, queries, heads, dim, dtype=q.dtype, device=device)
+    _require_cuda(k_codes=k_codes, out=out)
+    if out.dtype != q.dtype or tuple(out.shape) != (batch, queries, heads, dim):
+        raise RuntimeError(f"`out` must be a {q.dtype} tensor of shape {(batch, queries, heads, dim)}")
+    if not q.numel():
+        return out
+    need = _lib.check(_lib.lib.df11_kv_attention_workspace_bytes(batch, heads, kv_heads, queries, dim, slots, int(window)))
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    _lib.check(_lib.lib.df11_kv_attention(
+        q.data_ptr(), *q.stride()[:3], k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+        lengths.data_ptr(), lengths.numel(), first.data_ptr() if first is not None else None,
+        first.numel() if first is not None else 0, out.data_ptr(), workspace.data_ptr() if need else None, need, batch,
+        heads, kv_heads, queries, dim, slots, int(window), dim ** -0.5 if scale is None else float(scale),
+        _ELEMENT_TYPES[q.dtype], fmt, device.index, _stream(device)))
+    return out
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           out: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token per row of ``logits`` (``[rows, vocab]`` BF16, FP16 or FP32; rows may lie apart), int64 ``[rows]``.
+
+    ``uniform``: float32 ``[rows]`` in [0, 1), the only randomness.  The settings are numbers, or tensors of one entry
+    per row (float32; ``top_k`` int32).  The tokens are ordered by logit, descending, equal ones by index: ``top_k``
+    keeps the first so many (0: all), ``top_p`` those before which less than ``top_p`` of the mass that ``top_k`` left
+    lies (1: all), ``min_p`` those with at least ``min_p`` of the largest probability (0: all).  The result is the lowest
+    index at which the running mass of the kept tokens, in index order, exceeds ``uniform`` times their whole mass.
+    ``temperature`` 0 is arg-max, the lowest index among equals.  NaN and -inf are never drawn; a row of nothing else
+    gives 0 and sets ``STATUS_EMPTY_ROW`` in ``status``."""
+    if not logits.is_cuda:
+        raise RuntimeError(f"df11 kernels need CUDA tensors; `logits` is on {logits.device}")
+    device = logits.device
+    if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in _ELEMENT_TYPES:
+        raise RuntimeError("`logits` must be [rows, vocab] in bfloat16, float16 or float32")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise RuntimeError("the rows of `logits` must be contiguous")
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=device)
+    _require_cuda(uniform=uniform, out=out, status=status)
+    if uniform.device != device or uniform.dtype != torch.float32 or uniform.numel() != rows:
+        raise RuntimeError(f"`uniform` must be a float32 tensor of {rows} elements on {device}")
+    if out.device != device or out.dtype != torch.int64 or out.numel() != rows:
+        raise RuntimeError(f"`out` must be an int64 tensor of {rows} elements on {device}")
+    args = []
+    for name, value, dtype, fits in (("temperature", temperature, torch.float32, lambda x: 0 <= x < float("inf")),
+                                     ("top_k", top_k, torch.int32, lambda x: 0 <= x < 2 ** 31),
+                                     ("top_p", top_p, torch.float32, lambda x: 0 < x <= 1),
+                                     ("min_p", min_p, torch.float32, lambda x: 0 <= x <= 1)):
+        if isinstance(value, torch.Tensor):
+            _require_cuda(**{name: value})
+            if value.device != device or value.dtype != dtype or value.numel() != rows:
+                raise RuntimeError(f"`{name}` must be a number or a {dtype} tensor of {rows} elements on {device}")
+            args += [value.data_ptr(), 0]
+        else:
+            if not fits(value):
+                raise RuntimeError(f"`{name}` = {value} is out of range")
+            args += [None, int(value) if dtype == torch.int32 else float(value)]
+    if rows:
+        _lib.check(_lib.lib.df11_sample(
+            logits.data_ptr(), logits.stride(0), _ELEMENT_TYPES[logits.dtype], rows, vocab, uniform.data_ptr(), *args,
+            out.data_ptr(), status.data_ptr() if status is not None else None, device.index, _stream(device)))
     return out

@@ -43,6 +43,7 @@ extern "C" {
 #define DF11_STATUS_BAD_POSITIONS 2 /* output_positions not monotone / beyond n_elements    */
 #define DF11_STATUS_TRUNCATED 4    /* a format block holds more elements than max_block_elems */
 #define DF11_STATUS_TIMEOUT 8      /* a bounded wait for an asynchronous copy ran out        */
+#define DF11_STATUS_EMPTY_ROW 16   /* a row of logits with nothing to draw from (df11_sample) */
 
 /* Library version, major*10000 + minor*100 + patch.  (The reference keeps a format
  * version string, dfloat11.py:44; this number versions the ABI below.) */
@@ -373,6 +374,102 @@ int df11_encode_device_pack(const void *exponents, int64_t n_elements, const voi
                             const void *code_val, int32_t pad_len, uint32_t pad_val, void *workspace,
                             void *codes, int64_t n_bytes, void *gaps, int64_t n_gap_bytes,
                             void *positions, int64_t n_positions, int32_t device, void *stream);
+
+/*
+ * The key/value cache of a generation step, held in 8 bits.  No counterpart in the reference,
+ * which compresses weights only; once they are smaller, the cache is what fills the memory.
+ *
+ * Layout (all device memory, contiguous): codes [batch][kv_heads][max_slots][head_dim], one byte
+ * each; scales [batch][kv_heads][max_slots], float; one such pair for the keys and one for the
+ * values.  A row (one token of one head) x of largest magnitude a is stored as
+ *     DF11_KV_INT8   scale = a / 127, code = x * 127 / a to the nearest integer (ties to even)
+ *     DF11_KV_E4M3   scale = a / 448, code = x * 448 / a to the nearest e4m3 (ties to even)
+ * and stands for code * scale.  The code is the one of the exact quotient.  A row of zeros has
+ * scale 0; a row with an infinity or a NaN has scale NaN and codes 0 (it stands for NaNs).
+ */
+#define DF11_TYPE_BF16 0
+#define DF11_TYPE_FP16 1
+#define DF11_TYPE_FP32 2
+#define DF11_KV_INT8 0
+#define DF11_KV_E4M3 1
+#define DF11_KV_MAX_HEAD_DIM 256
+
+/*
+ * Quantises `tokens` new rows per sequence and head into the cache.
+ *   k, v        device, element_type (bf16 or fp16), [batch][kv_heads][tokens][head_dim] with any
+ *               strides (in elements) of the first three dimensions; head_dim is contiguous
+ *   positions   device, int64, n_positions (1 or batch) entries: token i of sequence b goes to
+ *               slot positions[b] + i.  A token whose slot is outside [0, max_slots) is not
+ *               written and sets DF11_STATUS_BAD_POSITIONS; all other slots keep their bytes.
+ *   head_dim    a multiple of 16, at most DF11_KV_MAX_HEAD_DIM; codes are 16-byte aligned
+ */
+int df11_kv_append(const void *k, const void *v, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t,
+                   int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, void *k_codes, void *k_scales,
+                   void *v_codes, void *v_scales, const void *positions, int64_t n_positions, int64_t batch,
+                   int32_t kv_heads, int64_t tokens, int32_t head_dim, int64_t max_slots,
+                   int32_t element_type, int32_t format, void *status, int32_t device, void *stream);
+
+/*
+ * Reads slots [first_slot, first_slot + n_slots) of every sequence and head back:
+ * k_out, v_out [batch][kv_heads][n_slots][head_dim] (contiguous, 16-byte aligned) receive code * scale, the product
+ * in fp32, rounded once to element_type (bf16 or fp16).
+ */
+int df11_kv_read(const void *k_codes, const void *k_scales, const void *v_codes, const void *v_scales,
+                 void *k_out, void *v_out, int64_t batch, int32_t kv_heads, int64_t max_slots,
+                 int32_t head_dim, int64_t first_slot, int64_t n_slots, int32_t element_type, int32_t format,
+                 int32_t device, void *stream);
+
+/*
+ * Attention of a few new tokens over the cache, read in its 8-bit form.
+ *   q         device, element_type (bf16 or fp16), [batch][heads][queries][head_dim] with any
+ *             strides (in elements) of the first three dimensions; heads is a multiple of kv_heads
+ *             and head h reads the keys of head h / (heads / kv_heads)
+ *   lengths   device, int64, n_lengths (1 or batch): filled slots, the new tokens' included.  Query
+ *             i stands at p = length - queries + i and sees slots t with low <= t <= p, where
+ *             low = max(first, p - window + 1) (window 0: low = first).  Slots outside
+ *             [0, max_slots) do not exist, whatever length and first say.
+ *   first     device, int64, n_first (1 or batch), or NULL for 0: slots before it are padding
+ *   out       [batch][queries][heads][head_dim], element_type, contiguous:
+ *             sum_t softmax_t(scale * q.k_t) v_t; zeros for a query that sees no slot
+ *   workspace device, 16-byte aligned, df11_kv_attention_workspace_bytes() bytes for the same
+ *             sizes (0 for some: NULL is fine then); used only while the call's kernels run, so
+ *             calls that may overlap need one each
+ * Sums and softmax statistics are fp32, in an order that depends on the sizes alone: the same call
+ * gives the same bits.
+ */
+int64_t df11_kv_attention_workspace_bytes(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
+                                          int32_t head_dim, int64_t max_slots, int32_t window);
+
+int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
+                      const void *k_codes, const void *k_scales, const void *v_codes, const void *v_scales,
+                      const void *lengths, int64_t n_lengths, const void *first, int64_t n_first, void *out,
+                      void *workspace, int64_t workspace_bytes, int64_t batch, int32_t heads,
+                      int32_t kv_heads, int64_t queries, int32_t head_dim, int64_t max_slots,
+                      int32_t window, float scale, int32_t element_type, int32_t format, int32_t device,
+                      void *stream);
+
+/*
+ * Draws one token per row of logits from given random numbers.
+ *   logits       device, element_type (bf16, fp16 or fp32), [rows][vocab], rows row_stride apart
+ *                (in elements)
+ *   uniform      device, float [rows], in [0, 1)
+ *   temperature, top_k, top_p, min_p   device, one entry per row (float, int32, float, float), or
+ *                NULL: then the *_value after it holds for all rows
+ *   out          device, int64 [rows]
+ * With p = softmax(logits / temperature) and the tokens ordered by logit, descending, equal ones by
+ * index: top_k keeps the first top_k (<= 0: all); top_p those before which less than top_p of the
+ * mass that top_k left lies (>= 1: all; always the first one); min_p those with p >= min_p * max p
+ * (<= 0: all).  The result is the lowest index at which the running mass of the kept tokens, in
+ * index order, exceeds uniform * their whole mass.  temperature <= 0 is arg-max (lowest index).  A
+ * NaN or -inf logit is never drawn; with +inf logits the draw is among those.  A row with nothing
+ * to draw gives 0 and sets DF11_STATUS_EMPTY_ROW in `status` (may be NULL).
+ * Masses are sums of 64-bit integers (weights relative to the largest, computed in fp64): exact,
+ * and the same in every order.  The reference leaves this to its caller's library.
+ */
+int df11_sample(const void *logits, int64_t row_stride, int32_t element_type, int64_t rows, int64_t vocab,
+                const void *uniform, const void *temperature, double temperature_value, const void *top_k,
+                int32_t top_k_value, const void *top_p, double top_p_value, const void *min_p,
+                double min_p_value, void *out, void *status, int32_t device, void *stream);
 
 #ifdef __cplusplus
 }
