@@ -31,14 +31,8 @@ __device__ __forceinline__ float warp_max(float x)
     return x;
 }
 
-__device__ __forceinline__ float warp_sum(float x)
-{
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-    return x;
-}
-
-// A length as the user's program may have it; what is beyond any cache must not overflow below.
+// A length or a first slot as the user's program may have it; what is beyond any cache must not
+// overflow in what is computed from it.
 __device__ __forceinline__ int64_t clamped_length(int64_t n) { return n < 0 ? 0 : n > (1ll << 40) ? 1ll << 40 : n; }
 
 struct Strides {
@@ -108,62 +102,540 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const uint8_t *k_codes, co
     for (int i = lane; i < dim; i += 32) out[i] = df11_from_float<T>(code_value(codes[i], format) * scale);
 }
 
-// One CTA of four warps per query row; a warp takes every fourth slot, one pass with a running
-// maximum and sum, and the warps' results are joined at the end.
-template <typename T>
-__global__ void __launch_bounds__(128) kv_attention_kernel(const T *q, Strides qs, const uint8_t *k_codes,
-                                                           const float *k_scales, const uint8_t *v_codes,
-                                                           const float *v_scales, const int64_t *lengths, int length_per,
-                                                           const int64_t *first, int first_per, T *out, int heads,
-                                                           int kv_heads, int64_t queries, int dim, int64_t max_slots,
-                                                           int window, float scale, int format)
+// ---------------------------------------------------------------------------------------------
+// Attention.  For a few query rows per key head the work is reading the cache once: 2 (d + 4) bytes
+// per slot against 4 d multiply-adds per row, so one pass, in which a code goes from memory to one
+// register, is widened to fp16 there (exactly: int8 and e4m3 are subsets of fp16) and meets the
+// matrix unit in that register.  Nothing passes through shared memory:
+//
+//   scores   S^T[16 slots x 8 rows] += K[16 x 16] Q^T[16 x 8]     (m16n8k16, fp32 sums)
+//   values   O^T[16 dims x 8 rows]  += V^T[16 x 16] P^T[16 x 8]
+//
+// The query rows are the narrow side, so a group of up to 8 rows wastes nothing.  A product may
+// number its inner dimension as it likes as long as both operands agree: a thread loads 16
+// consecutive bytes of a key row and calls them the elements that the fragment layout gives it (the
+// query fragments are loaded in the same order), and of a value row 16 consecutive bytes whose
+// dimensions become the rows of eight fragments.  The scores come out with the slots across lanes
+// and the rows across registers; an 8x8 transposition between registers (movmatrix) turns the
+// weights into the second product's operand.
+//
+// Scales.  A key's scale multiplies its score.  A value's scale multiplies its weight before that is
+// rounded to fp16; so that neither over- nor underflows, weights are held relative to a running
+// bound of weight * scale, per row, in powers of two (2^6 below which 2^-30 of the largest is still
+// distinguished).  The running maximum is renewed only when a weight outgrows 2^14: a vote per tile
+// instead of a reduction over lanes.  Query rows are scaled by a power of two to just below 2, which
+// fp16 holds exactly from there down to 2^-24; smaller entries are rounded to multiples of 2^-24 of that.
+// Sums, maxima and denominators are fp32.
+//
+// The slots of a sequence are divided among `cluster` CTAs that join their results through
+// distributed shared memory, and, for long caches with few heads, among several such clusters
+// whose results a second kernel joins in a fixed order.
+constexpr int kAttWarps = 4;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                            uint32_t b1)
 {
-    __shared__ float part_o[4][DF11_KV_MAX_HEAD_DIM], part_m[4], part_l[4];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t i = blockIdx.x % queries, h = blockIdx.x / queries % heads, b = blockIdx.x / queries / heads;
-    const int64_t cell0 = (b * kv_heads + h / (heads / kv_heads)) * max_slots;
-    const int64_t place = clamped_length(lengths[length_per ? b : 0]) - queries + i;
-    int64_t low = first ? first[first_per ? b : 0] : 0;
-    if (window > 0 && place - window + 1 > low) low = place - window + 1;
-    if (low < 0) low = 0;
-    const int64_t high = place < max_slots ? place : max_slots - 1;
-    constexpr int kPer = DF11_KV_MAX_HEAD_DIM / 32;
-    float x[kPer], o[kPer] = {};
-    for (int j = 0; j < kPer; ++j)
-        x[j] = lane + 32 * j < dim ? df11_to_float(q[b * qs.b + h * qs.h + i * qs.t + lane + 32 * j]) * scale : 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int64_t t = low + warp; t <= high; t += 4) {
-        const uint8_t *kc = k_codes + (cell0 + t) * dim, *vc = v_codes + (cell0 + t) * dim;
-        float s = 0.0f;
-        for (int j = 0; j < kPer; ++j)
-            if (lane + 32 * j < dim) s += x[j] * code_value(kc[lane + 32 * j], format);
-        s = warp_sum(s) * k_scales[cell0 + t];
-        const float peak = fmaxf(m, s), base = peak == -INFINITY ? 0.0f : peak;
-        const float old = expf(m - base), p = expf(s - base);
-        l = l * old + p;
-        const float w = p * v_scales[cell0 + t];
-        for (int j = 0; j < kPer; ++j) {
-            o[j] *= old;
-            if (lane + 32 * j < dim) o[j] += w * code_value(vc[lane + 32 * j], format);
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// Four codes to two pairs of fp16.  int8: the code plus 128 becomes the low mantissa bits of 1024.
+template <int FMT> __device__ __forceinline__ void widen(uint32_t codes, uint32_t &lo, uint32_t &hi)
+{
+    if (FMT == DF11_KV_INT8) {
+        const uint32_t u = codes ^ 0x80808080u;
+        const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
+        const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+        const __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&l), bias), b = __hsub2(*reinterpret_cast<const __half2 *>(&h), bias);
+        lo = *reinterpret_cast<const uint32_t *>(&a);
+        hi = *reinterpret_cast<const uint32_t *>(&b);
+    } else {
+        asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
+            : "=r"(lo), "=r"(hi)
+            : "r"(codes));
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_half(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
+
+template <int BYTES> struct Bytes;
+template <> struct Bytes<8> {
+    uint32_t w[2];
+    __device__ __forceinline__ void load(const uint8_t *p)
+    {
+        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = x.x, w[1] = x.y;
+    }
+};
+template <> struct Bytes<16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const uint8_t *p)
+    {
+        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    }
+};
+
+struct AttentionArgs {
+    const void *q;
+    Strides qs;
+    const uint8_t *k_codes, *v_codes;
+    const float *k_scales, *v_scales;
+    const int64_t *lengths, *first;
+    int length_per, first_per;
+    void *out;
+    float *workspace;                   // [unit][parts][rows * (D + 2)] where parts > 1
+    int kv_heads, group, dim, window, row_groups, cluster, parts, q_aligned;
+    int64_t queries, max_slots;
+    float scale;
+};
+
+// Where a query stands and the slots that it sees.
+struct Sight {
+    int64_t low, high;
+};
+__device__ __forceinline__ Sight sight_of(const AttentionArgs &a, int64_t length, int64_t first, int64_t query)
+{
+    const int64_t place = length - a.queries + query;
+    int64_t low = first;
+    if (a.window > 0 && place - a.window + 1 > low) low = place - a.window + 1;
+    return {low, place < a.max_slots ? place : a.max_slots - 1};
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_barrier()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float remote_load(const float *local, uint32_t rank)
+{
+    uint32_t addr = (uint32_t)__cvta_generic_to_shared(local), there;
+    float x;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(there));
+    return x;
+}
+
+// One CTA: up to NT * 8 query rows of one key head, and its share of the slots they see.
+template <int D, int NT, int FMT, typename T>
+__global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionArgs a)
+{
+    constexpr int kRows = NT * 8;
+    constexpr int kKeyChunks = D / 64;                      // 16-byte chunks of a key row per thread
+    constexpr int kValBytes = D >= 128 ? 16 : D / 8;        // consecutive bytes of a value row per thread
+    constexpr int kValChunks = D / 8 / kValBytes;
+    constexpr int kBlocks = D / 16;                         // fragments of 16 dimensions
+    extern __shared__ float shared[];
+    float *part_o = shared;                                 // [warps][rows][D]
+    float *part_m = part_o + kAttWarps * kRows * D;         // [warps][rows]
+    float *part_l = part_m + kAttWarps * kRows;
+    float *all_m = part_l + kAttWarps * kRows;              // [rows]
+    float *all_l = all_m + kRows;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    const int splits = a.cluster * a.parts;
+    const int64_t unit = blockIdx.x / splits;
+    const int split = blockIdx.x % splits;
+    const int64_t head = unit / a.row_groups, b = head / a.kv_heads;
+    const int h = (int)(head % a.kv_heads);
+    const int64_t row0 = unit % a.row_groups * kRows, rows = (int64_t)a.group * a.queries;
+    const int64_t last_row = min(row0 + kRows, rows) - 1;
+
+    // the query fragments, in the order in which the key bytes lie
+    uint32_t qf[NT][D / 16][2];
+    float mult[NT][2];                                      // score = sum * mult * key scale, in powers of two
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int64_t row = min(row0 + nt * 8 + r, rows - 1);
+        const T *x = (const T *)a.q + b * a.qs.b + (h * a.group + row % a.group) * a.qs.h + row / a.group * a.qs.t;
+        float peak = 0.0f;
+        uint32_t raw[D / 16][2];
+#pragma unroll
+        for (int j = 0; j < kKeyChunks; ++j) {
+            const int d0 = (j * 4 + c) * 16;
+            if (d0 >= a.dim) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) raw[j * 4 + w][0] = raw[j * 4 + w][1] = 0;
+            } else if (a.q_aligned) {
+                const uint4 lo = *reinterpret_cast<const uint4 *>(x + d0), hi = *reinterpret_cast<const uint4 *>(x + d0 + 8);
+                raw[j * 4][0] = lo.x, raw[j * 4][1] = lo.y, raw[j * 4 + 1][0] = lo.z, raw[j * 4 + 1][1] = lo.w;
+                raw[j * 4 + 2][0] = hi.x, raw[j * 4 + 2][1] = hi.y, raw[j * 4 + 3][0] = hi.z, raw[j * 4 + 3][1] = hi.w;
+            } else {
+                const uint16_t *y = reinterpret_cast<const uint16_t *>(x) + d0;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) raw[j * 4 + w / 2][w & 1] = (uint32_t)y[2 * w] | (uint32_t)y[2 * w + 1] << 16;
+            }
         }
-        m = peak;
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const T *pair = reinterpret_cast<const T *>(&raw[s][i]);
+                peak = fmaxf(peak, fmaxf(fabsf(df11_to_float(pair[0])), fabsf(df11_to_float(pair[1]))));
+            }
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+        peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+        // 2^e <= peak < 2^(e+1); an infinity stays one
+        const int e = peak > 0.0f && peak <= 3.402823466e38f ? max((int)(__float_as_uint(peak) >> 23) - 127, -126) : 0;
+        const float down = power_of_two(-e);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const T *pair = reinterpret_cast<const T *>(&raw[s][i]);
+                qf[nt][s][i] = pack_half(df11_to_float(pair[0]) * down, df11_to_float(pair[1]) * down);
+            }
+        const float up = power_of_two(e) * (a.scale * kLog2e);
+        mult[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c);          // the row of this thread's first column
+        mult[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
     }
-    for (int j = 0; j < kPer; ++j) part_o[warp][lane + 32 * j] = o[j];
-    if (lane == 0) part_m[warp] = m, part_l[warp] = l;
+
+    // the slots that any of the rows sees, and those that all of them see
+    const int64_t length = clamped_length(a.lengths[a.length_per ? b : 0]);
+    const int64_t start = a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
+    const Sight top = sight_of(a, length, start, row0 / a.group), bottom = sight_of(a, length, start, last_row / a.group);
+    const int64_t low = top.low, n = max(bottom.high - low + 1, (int64_t)0);
+    const int inner_low = (int)min(bottom.low - low, n), inner_high = (int)max(top.high - low, (int64_t)-1);
+    const int count = (int)n;
+    int col_low[NT][2], col_high[NT][2];                    // relative to `low`
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Sight s = sight_of(a, length, start, min(row0 + nt * 8 + 2 * c + i, rows - 1) / a.group);
+            col_low[nt][i] = (int)min(s.low - low, n);
+            col_high[nt][i] = (int)max(s.high - low, (int64_t)-1);
+        }
+
+    const int64_t tiles = (n + 15) / 16;
+    const int64_t begin = tiles * split / splits, end = tiles * (split + 1) / splits;
+    const int64_t cell0 = head * a.max_slots + low;
+
+    float o[kBlocks][NT][4] = {};
+    // running maximum, sum, factor on weight * scale, and the largest weight * scale when it was set;
+    // the factor starts so large that the first weight * scale that is not zero sets it
+    float m[NT][2], l[NT][2] = {}, f[NT][2], big[NT][2] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, f[nt][0] = f[nt][1] = 0x1p126f;
+
+    Bytes<16> kx[2][kKeyChunks];
+    Bytes<kValBytes> vx[4][kValChunks];
+    float ks[2], vs[2];
+    auto load_keys = [&](int64_t tile) {
+        const int s0 = (int)(tile * 16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int slot = s0 + r + 8 * i;
+            const bool in = slot < count;
+            const uint8_t *p = a.k_codes + (cell0 + slot) * a.dim;
+            ks[i] = in ? __ldg(a.k_scales + cell0 + slot) : 0.0f;
+            vs[i] = in ? __ldg(a.v_scales + cell0 + slot) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < kKeyChunks; ++j) {
+                kx[i][j] = {};
+                if (in && (j * 4 + c) * 16 < a.dim) kx[i][j].load(p + (j * 4 + c) * 16);
+            }
+        }
+    };
+    auto load_values = [&](int64_t tile) {
+        const int s0 = (int)(tile * 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int slot = s0 + 2 * c + (i & 1) + 8 * (i >> 1);
+            const uint8_t *p = a.v_codes + (cell0 + slot) * a.dim;
+#pragma unroll
+            for (int j = 0; j < kValChunks; ++j) {
+                vx[i][j] = {};
+                if (slot < count && (j * 8 + r) * kValBytes < a.dim) vx[i][j].load(p + (j * 8 + r) * kValBytes);
+            }
+        }
+    };
+
+    int64_t tile = begin + warp;
+    if (tile < end) load_keys(tile), load_values(tile);
+    for (; tile < end; tile += kAttWarps) {
+        const bool more = tile + kAttWarps < end;
+        float s[NT][4] = {};
+#pragma unroll
+        for (int j = 0; j < kKeyChunks; ++j)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t a0, a1, a2, a3;
+                widen<FMT>(kx[0][j].w[w], a0, a2);
+                widen<FMT>(kx[1][j].w[w], a1, a3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[nt], a0, a1, a2, a3, qf[nt][j * 4 + w][0], qf[nt][j * 4 + w][1]);
+            }
+        const float key_scale[2] = {ks[0], ks[1]}, value_scale[2] = {vs[0], vs[1]};
+        if (more) load_keys(tile + kAttWarps);
+
+        const int s0 = (int)(tile * 16);
+        const bool whole = s0 >= inner_low && s0 + 15 <= inner_high;    // every row sees every slot
+        float p[NT][4], w[NT][4];
+        auto weigh = [&]() {                                            // true if a weight has outgrown its bound
+            bool over = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int col = i & 1, slot = s0 + r + 8 * (i >> 1);
+                    p[nt][i] = exp2f(s[nt][i] - m[nt][col]);
+                    w[nt][i] = p[nt][i] * value_scale[i >> 1] * f[nt][col];
+                    if (!whole && (slot < col_low[nt][col] || slot > col_high[nt][col])) p[nt][i] = w[nt][i] = 0.0f;
+                    over |= fmaxf(p[nt][i], w[nt][i]) > 16384.0f;
+                }
+            return over;
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[nt][i] *= key_scale[i >> 1] * mult[nt][i & 1];
+        if (__any_sync(0xffffffffu, weigh())) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int col = 0; col < 2; ++col) {
+                    float peak = m[nt][col];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int slot = s0 + r + 8 * i;
+                        if (whole || (slot >= col_low[nt][col] && slot <= col_high[nt][col])) peak = fmaxf(peak, s[nt][col + 2 * i]);
+                    }
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, x));
+                    const float was = m[nt][col];
+                    const float back = was == -INFINITY ? 0.0f : exp2f(was - peak);
+                    float heavy = 0.0f;                                  // the largest weight * scale, relative to `peak`
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int slot = s0 + r + 8 * i;
+                        if (whole || (slot >= col_low[nt][col] && slot <= col_high[nt][col]))
+                            heavy = fmaxf(heavy, exp2f(s[nt][col + 2 * i] - peak) * value_scale[i]);
+                    }
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) heavy = fmaxf(heavy, __shfl_xor_sync(0xffffffffu, heavy, x));
+                    heavy = fmaxf(heavy, big[nt][col] * back);
+                    // f brings it to [2^6, 2^7)
+                    const float now = heavy > 0.0f && heavy <= 3.402823466e38f
+                        ? power_of_two(133 - (int)(__float_as_uint(heavy) >> 23)) : f[nt][col];
+                    const float turn = back * (now / f[nt][col]);
+                    l[nt][col] *= back;
+#pragma unroll
+                    for (int k = 0; k < kBlocks; ++k) o[k][nt][col] *= turn, o[k][nt][col + 2] *= turn;
+                    m[nt][col] = peak, big[nt][col] = heavy, f[nt][col] = now;
+                }
+            weigh();
+        }
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            l[nt][0] += p[nt][0] + p[nt][2];
+            l[nt][1] += p[nt][1] + p[nt][3];
+            pb[nt][0] = transpose_8x8(pack_half(w[nt][0], w[nt][1]));
+            pb[nt][1] = transpose_8x8(pack_half(w[nt][2], w[nt][3]));
+        }
+#pragma unroll
+        for (int j = 0; j < kValChunks; ++j)
+#pragma unroll
+            for (int x = 0; x < kValBytes / 4; ++x)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t pick = half ? 0x7362 : 0x5140;       // two dimensions of two slots
+                    uint32_t a0, a1, a2, a3;
+                    widen<FMT>(__byte_perm(vx[0][j].w[x], vx[1][j].w[x], pick), a0, a1);
+                    widen<FMT>(__byte_perm(vx[2][j].w[x], vx[3][j].w[x], pick), a2, a3);
+                    const int k = (j * (kValBytes / 4) + x) * 2 + half;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[k][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                }
+        if (more) load_values(tile + kAttWarps);
+    }
+
+    // the warps' results are joined
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[nt][col] += __shfl_xor_sync(0xffffffffu, l[nt][col], x);
+            if (r == 0) {
+                part_m[warp * kRows + nt * 8 + 2 * c + col] = m[nt][col];
+                part_l[warp * kRows + nt * 8 + 2 * c + col] = l[nt][col];
+            }
+        }
     __syncthreads();
-    float peak = fmaxf(fmaxf(part_m[0], part_m[1]), fmaxf(part_m[2], part_m[3]));
-    if (peak == -INFINITY) peak = 0.0f;
-    float total = 0.0f, w[4];
-    for (int k = 0; k < 4; ++k) {
-        w[k] = expf(part_m[k] - peak);
-        total += w[k] * part_l[k];
+    if (threadIdx.x < kRows) {
+        float peak = -INFINITY, total = 0.0f;
+        for (int k = 0; k < kAttWarps; ++k) peak = fmaxf(peak, part_m[k * kRows + threadIdx.x]);
+        for (int k = 0; k < kAttWarps; ++k) {
+            const float x = part_m[k * kRows + threadIdx.x];
+            if (x != -INFINITY) total += exp2f(x - peak) * part_l[k * kRows + threadIdx.x];
+            else total += part_l[k * kRows + threadIdx.x];      // nothing, or a NaN
+        }
+        all_m[threadIdx.x] = peak;
+        all_l[threadIdx.x] = total;
     }
-    T *row = out + ((b * queries + i) * heads + h) * dim;
-    for (int c = threadIdx.x; c < dim; c += 128) {
-        float sum = 0.0f;
-        for (int k = 0; k < 4; ++k) sum += w[k] * part_o[k][c];
-        row[c] = df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int col = 0; col < 2; ++col) {
+            const int row = nt * 8 + 2 * c + col;
+            const float turn = m[nt][col] == -INFINITY ? 1.0f : exp2f(m[nt][col] - all_m[row]) / f[nt][col];
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) {
+                // fragment k: this thread's bytes 2k and 2k + 1 of its chunk
+                const int byte = 2 * k % kValBytes, d0 = ((2 * k / kValBytes) * 8 + r) * kValBytes + byte;
+                part_o[(warp * kRows + row) * D + d0] = o[k][nt][col] * turn;
+                part_o[(warp * kRows + row) * D + d0 + 1] = o[k][nt][col + 2] * turn;
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kRows * D; i += kAttWarps * 32) {
+        float sum = part_o[i];
+        for (int k = 1; k < kAttWarps; ++k) sum += part_o[k * kRows * D + i];
+        part_o[i] = sum;
     }
+
+    // the CTAs' results are joined, a share of the numbers by each CTA
+    const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0;
+    if (a.cluster > 1) cluster_barrier();
+    else __syncthreads();
+    const int part = split / a.cluster;
+    float *ws = a.parts > 1 ? a.workspace + (unit * a.parts + part) * (kRows * (D + 2)) : nullptr;
+    for (int i = (int)rank * kAttWarps * 32 + threadIdx.x; i < kRows * D; i += a.cluster * kAttWarps * 32) {
+        const int row = i / D, d = i % D;
+        if (row0 + row > last_row || d >= a.dim) continue;
+        float peak = -INFINITY, total = 0.0f, sum = 0.0f;
+        if (a.cluster == 1) {
+            peak = all_m[row], total = all_l[row], sum = part_o[i];
+        } else {
+            for (int k = 0; k < a.cluster; ++k) peak = fmaxf(peak, remote_load(all_m + row, k));
+            for (int k = 0; k < a.cluster; ++k) {
+                const float x = remote_load(all_m + row, k), turn = x == -INFINITY ? 1.0f : exp2f(x - peak);
+                total += turn * remote_load(all_l + row, k);
+                sum += turn * remote_load(part_o + i, k);
+            }
+        }
+        if (a.parts > 1) {
+            ws[i] = sum;
+            if (d == 0) ws[kRows * D + row] = peak, ws[kRows * D + kRows + row] = total;
+        } else {
+            const int64_t at = row0 + row, query = at / a.group, hq = h * a.group + at % a.group;
+            ((T *)a.out)[((b * a.queries + query) * (a.kv_heads * a.group) + hq) * a.dim + d] =
+                df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
+        }
+    }
+    if (a.cluster > 1) cluster_barrier();               // nobody leaves while its memory is read
+}
+
+// Joins the clusters' results: one CTA per query row.
+template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_attention_join_kernel(AttentionArgs a)
+{
+    constexpr int kRows = NT * 8;
+    const int64_t rows = (int64_t)a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
+    const int row = (int)(at % kRows), d = threadIdx.x;
+    const float *ws = a.workspace + (head * a.row_groups + at / kRows) * a.parts * (kRows * (D + 2));
+    if (d >= a.dim) return;
+    float peak = -INFINITY, total = 0.0f, sum = 0.0f;
+    for (int k = 0; k < a.parts; ++k) peak = fmaxf(peak, ws[k * (kRows * (D + 2)) + kRows * D + row]);
+    for (int k = 0; k < a.parts; ++k) {
+        const float *part = ws + k * (kRows * (D + 2));
+        const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2f(x - peak);
+        total += turn * part[kRows * D + kRows + row];
+        sum += turn * part[row * D + d];
+    }
+    const int64_t hq = head % a.kv_heads * a.group + at % a.group;
+    ((T *)a.out)[((b * a.queries + at / a.group) * (a.kv_heads * a.group) + hq) * a.dim + d] =
+        df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
+}
+
+// How a call is divided, from its sizes alone.
+struct Division {
+    int width, tiles_n, cluster, parts;     // padded head_dim, row tiles of 8, CTAs per cluster, clusters per unit
+    int64_t row_groups, units;
+};
+
+Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries, int32_t head_dim, int64_t max_slots, int32_t window)
+{
+    Division d;
+    const int64_t rows = (int64_t)(heads / kv_heads) * queries;
+    d.width = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
+    d.tiles_n = rows > 8 && d.width < 256 ? 2 : 1;
+    d.row_groups = (rows + d.tiles_n * 8 - 1) / (d.tiles_n * 8);
+    d.units = batch * kv_heads * d.row_groups;
+    const int64_t span = window > 0 && window + queries < max_slots ? window + queries : max_slots;
+    const int64_t tiles = (span + 15) / 16, most = (tiles + 2 * kAttWarps - 1) / (2 * kAttWarps);   // two tiles per warp
+    int64_t want = (900 + d.units - 1) / (d.units > 0 ? d.units : 1);
+    if (want > most) want = most;
+    d.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
+    d.parts = 1;
+    if (want > 8 && tiles > 8 * 64) d.parts = (int)((want + 7) / 8);
+    return d;
+}
+
+template <int D, int NT, int FMT, typename T>
+cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStream_t stream)
+{
+    constexpr int kRows = NT * 8;
+    constexpr size_t kShared = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
+    auto kernel = kv_attention_kernel<D, NT, FMT, T>;
+    if (kShared > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(d.units * d.cluster * d.parts));
+    config.blockDim = dim3(kAttWarps * 32);
+    config.dynamicSmemBytes = kShared;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)d.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
+    if (e != cudaSuccess || d.parts == 1) return e;
+    const int64_t heads = d.units / d.row_groups;
+    kv_attention_join_kernel<D, NT, T><<<(unsigned)(heads * a.group * a.queries), D, 0, stream>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, cudaStream_t stream)
+{
+#define DF11_ATTENTION(D, NT)                                                                     \
+    if (d.width == D && d.tiles_n == NT)                                                          \
+        return format == DF11_KV_INT8 ? launch_attention<D, NT, DF11_KV_INT8, T>(a, d, stream)    \
+                                      : launch_attention<D, NT, DF11_KV_E4M3, T>(a, d, stream);
+    DF11_ATTENTION(64, 1)
+    DF11_ATTENTION(64, 2)
+    DF11_ATTENTION(128, 1)
+    DF11_ATTENTION(128, 2)
+    DF11_ATTENTION(256, 1)
+#undef DF11_ATTENTION
+    return cudaErrorInvalidValue;
 }
 
 int check_cache(const void *kc, const void *ks, const void *vc, const void *vs, int64_t batch, int32_t kv_heads,
@@ -258,8 +730,13 @@ extern "C" int df11_kv_read(const void *k_codes, const void *k_scales, const voi
 extern "C" int64_t df11_kv_attention_workspace_bytes(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
                                                      int32_t head_dim, int64_t max_slots, int32_t window)
 {
-    (void)batch, (void)heads, (void)kv_heads, (void)queries, (void)head_dim, (void)max_slots, (void)window;
-    return 0;
+    if (batch < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || queries < 0 || max_slots < 1 || window < 0)
+        return df11_fail(DF11_ERR_BADARG, "batch, heads, queries, max_slots or window out of range");
+    if (head_dim < 16 || head_dim > DF11_KV_MAX_HEAD_DIM || head_dim % 16)
+        return df11_fail(DF11_ERR_BADARG, "head_dim %d: multiples of 16 up to %d are supported", head_dim, DF11_KV_MAX_HEAD_DIM);
+    if ((double)batch * heads * (double)queries > 2e9) return df11_fail(DF11_ERR_BADARG, "too many query rows for one call");
+    const Division d = divide(batch, heads, kv_heads, queries, head_dim, max_slots, window);
+    return d.parts > 1 ? d.units * d.parts * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float) : 0;
 }
 
 extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
@@ -286,16 +763,21 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     if (rows == 0) return DF11_OK;
     Df11DeviceScope scope(device);
     if (!scope.ok) return df11_fail(DF11_ERR_CUDA, "cudaSetDevice(%d) failed", device);
-    const Strides qs = {q_stride_b, q_stride_h, q_stride_t};
-    if (element_type == DF11_TYPE_BF16)
-        kv_attention_kernel<<<(unsigned)rows, 128, 0, (cudaStream_t)stream>>>(
-            (const __nv_bfloat16 *)q, qs, (const uint8_t *)k_codes, (const float *)k_scales, (const uint8_t *)v_codes,
-            (const float *)v_scales, (const int64_t *)lengths, n_lengths > 1, (const int64_t *)first, n_first > 1,
-            (__nv_bfloat16 *)out, heads, kv_heads, queries, head_dim, max_slots, window, scale, format);
-    else
-        kv_attention_kernel<<<(unsigned)rows, 128, 0, (cudaStream_t)stream>>>(
-            (const __half *)q, qs, (const uint8_t *)k_codes, (const float *)k_scales, (const uint8_t *)v_codes,
-            (const float *)v_scales, (const int64_t *)lengths, n_lengths > 1, (const int64_t *)first, n_first > 1,
-            (__half *)out, heads, kv_heads, queries, head_dim, max_slots, window, scale, format);
-    return launched();
+    const Division d = divide(batch, heads, kv_heads, queries, head_dim, max_slots, window);
+    if ((double)d.units * d.cluster * d.parts > 2e9) return df11_fail(DF11_ERR_BADARG, "too many query rows for one call");
+    AttentionArgs a = {};
+    a.q = q, a.qs = {q_stride_b, q_stride_h, q_stride_t};
+    a.q_aligned = !(((uintptr_t)q & 15) || (q_stride_b | q_stride_h | q_stride_t) & 7);
+    a.k_codes = (const uint8_t *)k_codes, a.v_codes = (const uint8_t *)v_codes;
+    a.k_scales = (const float *)k_scales, a.v_scales = (const float *)v_scales;
+    a.lengths = (const int64_t *)lengths, a.length_per = n_lengths > 1;
+    a.first = (const int64_t *)first, a.first_per = n_first > 1;
+    a.out = out, a.workspace = (float *)workspace;
+    a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = head_dim, a.window = window;
+    a.row_groups = (int)d.row_groups, a.cluster = d.cluster, a.parts = d.parts;
+    a.queries = queries, a.max_slots = max_slots, a.scale = scale;
+    const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, (cudaStream_t)stream)
+                                                         : launch_attention<__half>(a, d, format, (cudaStream_t)stream);
+    if (e != cudaSuccess) return df11_fail(DF11_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
+    return DF11_OK;
 }

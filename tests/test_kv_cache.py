@@ -285,6 +285,20 @@ def test_attention_flat_over_values_of_very_different_size():
 
 
 @gpu
+def test_attention_values_that_start_with_zeros():
+    """A sequence whose first values are zeros and whose others are tiny or huge; and one that is all zeros."""
+    cache = filled_cache(3, 1, 500, 64, "e4m3", seed=30)
+    for b, size in ((0, 2.0 ** -40), (1, 2.0 ** 40), (2, 0.0)):
+        cache[3][b, :, :100] = 0
+        cache[3][b, :, 100:] *= size
+    q = query(3, 4, 1, 64, torch.bfloat16, 31)
+    lengths = torch.tensor([500, 480, 300], device=DEV)
+    got = ops.kv_attention(q, *cache, lengths).double().cpu()
+    want, bound = reference_attention(q, cache, lengths.tolist(), [0] * 3, 0.125, 0)
+    assert ((got - want).abs() <= bound + want.abs() * 2.0 ** -8).all() and not got[2].any() and got[0].any()
+
+
+@gpu
 def test_attention_lengths_beyond_the_cache_and_shared_ones():
     cache = filled_cache(3, 2, 96, 128, "int8", seed=16)
     q = query(3, 8, 1, 128, torch.bfloat16, 17)
@@ -294,7 +308,10 @@ def test_attention_lengths_beyond_the_cache_and_shared_ones():
     assert torch.equal(got, many)
     check_attention(q, cache, torch.tensor([97, 120, 10 ** 6], device=DEV))
     check_attention(q, cache, torch.tensor([-1, -2 ** 63, 50], device=DEV))
-    assert not ops.kv_attention(q, *cache, one, first=torch.tensor([2 ** 62], device=DEV)).any()
+    for first in (2 ** 62, 2 ** 63 - 1):
+        for length in (one, torch.tensor([-5], device=DEV), torch.tensor([2 ** 63 - 1], device=DEV)):
+            assert not ops.kv_attention(q, *cache, length, first=torch.tensor([first], device=DEV)).any()
+    check_attention(q, cache, one, first=torch.tensor([-2 ** 63], device=DEV))
 
 
 @gpu
