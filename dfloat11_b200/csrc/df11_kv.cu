@@ -148,21 +148,28 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x)
     return y;
 }
 
-// Four codes to two pairs of fp16.  int8: the code plus 128 becomes the low mantissa bits of 1024.
+// Four codes to two pairs of fp16.  int8: the code plus 128 becomes the bits of a subnormal, so the
+// pair stands for (code + 128) 2^-24, exactly; the products' sums are put right by 128 times the sum of
+// the other operand.  e4m3: the value itself.
+constexpr float kInt8Unit = 0x1p24f;
 template <int FMT> __device__ __forceinline__ void widen(uint32_t codes, uint32_t &lo, uint32_t &hi)
 {
     if (FMT == DF11_KV_INT8) {
         const uint32_t u = codes ^ 0x80808080u;
-        const __half2 bias = __half2half2(__ushort_as_half(0x6480));  // 1152
-        const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
-        const __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&l), bias), b = __hsub2(*reinterpret_cast<const __half2 *>(&h), bias);
-        lo = *reinterpret_cast<const uint32_t *>(&a);
-        hi = *reinterpret_cast<const uint32_t *>(&b);
+        lo = __byte_perm(u, 0, 0x4140);
+        hi = __byte_perm(u, 0, 0x4342);
     } else {
         asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
             : "=r"(lo), "=r"(hi)
             : "r"(codes));
     }
+}
+
+__device__ __forceinline__ float exp2_approx(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t pack_half(float a, float b)
@@ -229,18 +236,40 @@ __device__ __forceinline__ void cluster_barrier()
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
+__device__ __forceinline__ uint32_t remote_address(const float *local, uint32_t rank)
+{
+    uint32_t there;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    return there;
+}
+
 __device__ __forceinline__ float remote_load(const float *local, uint32_t rank)
 {
-    uint32_t addr = (uint32_t)__cvta_generic_to_shared(local), there;
     float x;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(there));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote_address(local, rank)));
     return x;
 }
 
+__device__ __forceinline__ float4 remote_load4(const float *local, uint32_t rank)
+{
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(remote_address(local, rank)));
+    return x;
+}
+
+template <typename T> __device__ __forceinline__ void store4(T *p, float4 x)
+{
+    T y[4] = {df11_from_float<T>(x.x), df11_from_float<T>(x.y), df11_from_float<T>(x.z), df11_from_float<T>(x.w)};
+    *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(y);
+}
+
 // One CTA: up to NT * 8 query rows of one key head, and its share of the slots they see.
-template <int D, int NT, int FMT, typename T>
-__global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionArgs a)
+// EXACT: head_dim is D; otherwise it is smaller, and what is loaded beyond it is some other chunk of the
+// same row that meets a zero of the query or ends in a result that nobody reads.
+template <int D, int NT, int FMT, bool EXACT, typename T>
+__global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) kv_attention_kernel(AttentionArgs a)
 {
     constexpr int kRows = NT * 8;
     constexpr int kKeyChunks = D / 64;                      // 16-byte chunks of a key row per thread
@@ -266,6 +295,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
     // the query fragments, in the order in which the key bytes lie
     uint32_t qf[NT][D / 16][2];
     float mult[NT][2];                                      // score = sum * mult * key scale, in powers of two
+    float offset[NT][2] = {};                               // what the sum starts from: - 128 sum(q) in the codes' unit
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int64_t row = min(row0 + nt * 8 + r, rows - 1);
@@ -307,7 +337,22 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
                 const T *pair = reinterpret_cast<const T *>(&raw[s][i]);
                 qf[nt][s][i] = pack_half(df11_to_float(pair[0]) * down, df11_to_float(pair[1]) * down);
             }
-        const float up = power_of_two(e) * (a.scale * kLog2e);
+        if (FMT == DF11_KV_INT8) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float2 pair = __half22float2(*reinterpret_cast<const __half2 *>(&qf[nt][s][i]));
+                    sum += pair.x + pair.y;
+                }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum *= -128.0f / kInt8Unit;
+            offset[nt][0] = __shfl_sync(0xffffffffu, sum, 8 * c);
+            offset[nt][1] = __shfl_sync(0xffffffffu, sum, 8 * c + 4);
+        }
+        const float up = power_of_two(e) * (a.scale * kLog2e) * (FMT == DF11_KV_INT8 ? kInt8Unit : 1.0f);
         mult[nt][0] = __shfl_sync(0xffffffffu, up, 8 * c);          // the row of this thread's first column
         mult[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
     }
@@ -330,10 +375,10 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
         }
 
     const int64_t tiles = (n + 15) / 16;
-    const int64_t begin = tiles * split / splits, end = tiles * (split + 1) / splits;
+    const int begin = (int)(tiles * split / splits), end = (int)(tiles * (split + 1) / splits);
     const int64_t cell0 = head * a.max_slots + low;
 
-    float o[kBlocks][NT][4] = {};
+    float o[kBlocks][NT][4] = {}, o128[NT][4] = {};         // o128: 128 times the sum of the weights, in the codes' unit
     // running maximum, sum, factor on weight * scale, and the largest weight * scale when it was set;
     // the factor starts so large that the first weight * scale that is not zero sets it
     float m[NT][2], l[NT][2] = {}, f[NT][2], big[NT][2] = {};
@@ -343,41 +388,48 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
     Bytes<16> kx[2][kKeyChunks];
     Bytes<kValBytes> vx[4][kValChunks];
     float ks[2], vs[2];
-    auto load_keys = [&](int64_t tile) {
-        const int s0 = (int)(tile * 16);
+    const int dim = EXACT ? D : a.dim;
+    // a thread's places in a tile of 16 slots: key rows r and r + 8, value rows 2c, 2c + 1, 2c + 8, 2c + 9
+    int key_at[kKeyChunks], value_at[kValChunks];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int slot = s0 + r + 8 * i;
-            const bool in = slot < count;
-            const uint8_t *p = a.k_codes + (cell0 + slot) * a.dim;
-            ks[i] = in ? __ldg(a.k_scales + cell0 + slot) : 0.0f;
-            vs[i] = in ? __ldg(a.v_scales + cell0 + slot) : 0.0f;
+    for (int j = 0; j < kKeyChunks; ++j) key_at[j] = EXACT ? j * 64 : min((j * 4 + c) * 16, dim - 16);
 #pragma unroll
-            for (int j = 0; j < kKeyChunks; ++j) {
-                kx[i][j] = {};
-                if (in && (j * 4 + c) * 16 < a.dim) kx[i][j].load(p + (j * 4 + c) * 16);
-            }
+    for (int j = 0; j < kValChunks; ++j) value_at[j] = EXACT ? j * 8 * kValBytes : min((j * 8 + r) * kValBytes, dim - kValBytes);
+    const uint8_t *const key_base = a.k_codes + cell0 * dim + (EXACT ? c * 16 : 0);
+    const uint8_t *const value_base = a.v_codes + cell0 * dim + (EXACT ? r * kValBytes : 0);
+    const float *const key_scales = a.k_scales + cell0, *const value_scales = a.v_scales + cell0;
+    // Past the last slot the last one is loaded again: its weight is 0 there, and whatever lies in the
+    // cache behind it (a NaN, say) does not reach a product.
+    auto load_keys = [&](int tile) {
+        const uint8_t *p = key_base + (int64_t)tile * 16 * dim;
+        const int s0 = tile * 16, left = count - 1 - s0;
+        const int r0 = left < 15 ? min(r, left) : r, r1 = left < 15 ? min(r + 8, left) : r + 8;
+        ks[0] = __ldg(key_scales + s0 + r0), ks[1] = __ldg(key_scales + s0 + r1);
+        vs[0] = __ldg(value_scales + s0 + r0), vs[1] = __ldg(value_scales + s0 + r1);
+#pragma unroll
+        for (int j = 0; j < kKeyChunks; ++j) {
+            kx[0][j].load(p + r0 * dim + key_at[j]);
+            kx[1][j].load(p + r1 * dim + key_at[j]);
         }
     };
-    auto load_values = [&](int64_t tile) {
-        const int s0 = (int)(tile * 16);
+    auto load_values = [&](int tile) {
+        const uint8_t *p = value_base + (int64_t)tile * 16 * dim;
+        const int left = count - 1 - tile * 16;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int slot = s0 + 2 * c + (i & 1) + 8 * (i >> 1);
-            const uint8_t *p = a.v_codes + (cell0 + slot) * a.dim;
+            const int at = 2 * c + (i & 1) + 8 * (i >> 1), row = left < 15 ? min(at, left) : at;
 #pragma unroll
-            for (int j = 0; j < kValChunks; ++j) {
-                vx[i][j] = {};
-                if (slot < count && (j * 8 + r) * kValBytes < a.dim) vx[i][j].load(p + (j * 8 + r) * kValBytes);
-            }
+            for (int j = 0; j < kValChunks; ++j) vx[i][j].load(p + row * dim + value_at[j]);
         }
     };
 
-    int64_t tile = begin + warp;
+    int tile = begin + warp;
     if (tile < end) load_keys(tile), load_values(tile);
     for (; tile < end; tile += kAttWarps) {
         const bool more = tile + kAttWarps < end;
-        float s[NT][4] = {};
+        float s[NT][4], s2[NT][4] = {};                     // two chains of sums: a product waits for the last of its chain
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][2] = offset[nt][0], s[nt][1] = s[nt][3] = offset[nt][1];
 #pragma unroll
         for (int j = 0; j < kKeyChunks; ++j)
 #pragma unroll
@@ -386,12 +438,12 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
                 widen<FMT>(kx[0][j].w[w], a0, a2);
                 widen<FMT>(kx[1][j].w[w], a1, a3);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) mma_16x8x16(s[nt], a0, a1, a2, a3, qf[nt][j * 4 + w][0], qf[nt][j * 4 + w][1]);
+                for (int nt = 0; nt < NT; ++nt) mma_16x8x16(w & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][j * 4 + w][0], qf[nt][j * 4 + w][1]);
             }
         const float key_scale[2] = {ks[0], ks[1]}, value_scale[2] = {vs[0], vs[1]};
         if (more) load_keys(tile + kAttWarps);
 
-        const int s0 = (int)(tile * 16);
+        const int s0 = tile * 16;
         const bool whole = s0 >= inner_low && s0 + 15 <= inner_high;    // every row sees every slot
         float p[NT][4], w[NT][4];
         auto weigh = [&]() {                                            // true if a weight has outgrown its bound
@@ -401,7 +453,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int col = i & 1, slot = s0 + r + 8 * (i >> 1);
-                    p[nt][i] = exp2f(s[nt][i] - m[nt][col]);
+                    p[nt][i] = exp2_approx(s[nt][i] - m[nt][col]);
                     w[nt][i] = p[nt][i] * value_scale[i >> 1] * f[nt][col];
                     if (!whole && (slot < col_low[nt][col] || slot > col_high[nt][col])) p[nt][i] = w[nt][i] = 0.0f;
                     over |= fmaxf(p[nt][i], w[nt][i]) > 16384.0f;
@@ -411,7 +463,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[nt][i] *= key_scale[i >> 1] * mult[nt][i & 1];
+            for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * (key_scale[i >> 1] * mult[nt][i & 1]);
         if (__any_sync(0xffffffffu, weigh())) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -426,13 +478,13 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, x));
                     const float was = m[nt][col];
-                    const float back = was == -INFINITY ? 0.0f : exp2f(was - peak);
+                    const float back = was == -INFINITY ? 0.0f : exp2_approx(was - peak);
                     float heavy = 0.0f;                                  // the largest weight * scale, relative to `peak`
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int slot = s0 + r + 8 * i;
                         if (whole || (slot >= col_low[nt][col] && slot <= col_high[nt][col]))
-                            heavy = fmaxf(heavy, exp2f(s[nt][col + 2 * i] - peak) * value_scale[i]);
+                            heavy = fmaxf(heavy, exp2_approx(s[nt][col + 2 * i] - peak) * value_scale[i]);
                     }
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) heavy = fmaxf(heavy, __shfl_xor_sync(0xffffffffu, heavy, x));
@@ -444,6 +496,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
                     l[nt][col] *= back;
 #pragma unroll
                     for (int k = 0; k < kBlocks; ++k) o[k][nt][col] *= turn, o[k][nt][col + 2] *= turn;
+                    o128[nt][col] *= turn;
                     m[nt][col] = peak, big[nt][col] = heavy, f[nt][col] = now;
                 }
             weigh();
@@ -455,6 +508,7 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
             l[nt][1] += p[nt][1] + p[nt][3];
             pb[nt][0] = transpose_8x8(pack_half(w[nt][0], w[nt][1]));
             pb[nt][1] = transpose_8x8(pack_half(w[nt][2], w[nt][3]));
+            if (FMT == DF11_KV_INT8) mma_16x8x16(o128[nt], 0x00800080u, 0x00800080u, 0x00800080u, 0x00800080u, pb[nt][0], pb[nt][1]);
         }
 #pragma unroll
         for (int j = 0; j < kValChunks; ++j)
@@ -491,32 +545,39 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
         for (int k = 0; k < kAttWarps; ++k) peak = fmaxf(peak, part_m[k * kRows + threadIdx.x]);
         for (int k = 0; k < kAttWarps; ++k) {
             const float x = part_m[k * kRows + threadIdx.x];
-            if (x != -INFINITY) total += exp2f(x - peak) * part_l[k * kRows + threadIdx.x];
+            if (x != -INFINITY) total += exp2_approx(x - peak) * part_l[k * kRows + threadIdx.x];
             else total += part_l[k * kRows + threadIdx.x];      // nothing, or a NaN
         }
         all_m[threadIdx.x] = peak;
         all_l[threadIdx.x] = total;
     }
     __syncthreads();
+    const int live = (int)(last_row - row0 + 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int col = 0; col < 2; ++col) {
             const int row = nt * 8 + 2 * c + col;
-            const float turn = m[nt][col] == -INFINITY ? 1.0f : exp2f(m[nt][col] - all_m[row]) / f[nt][col];
+            if (row >= live) continue;
+            const float turn = (m[nt][col] == -INFINITY ? 1.0f : exp2_approx(m[nt][col] - all_m[row]) / f[nt][col]) *
+                               (FMT == DF11_KV_INT8 ? kInt8Unit : 1.0f);
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 // fragment k: this thread's bytes 2k and 2k + 1 of its chunk
                 const int byte = 2 * k % kValBytes, d0 = ((2 * k / kValBytes) * 8 + r) * kValBytes + byte;
-                part_o[(warp * kRows + row) * D + d0] = o[k][nt][col] * turn;
-                part_o[(warp * kRows + row) * D + d0 + 1] = o[k][nt][col + 2] * turn;
+                *reinterpret_cast<float2 *>(part_o + (warp * kRows + row) * D + d0) =
+                    make_float2((o[k][nt][col] - o128[nt][col]) * turn, (o[k][nt][col + 2] - o128[nt][col]) * turn);
             }
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < kRows * D; i += kAttWarps * 32) {
-        float sum = part_o[i];
-        for (int k = 1; k < kAttWarps; ++k) sum += part_o[k * kRows * D + i];
-        part_o[i] = sum;
+    for (int i = threadIdx.x * 4; i < live * D; i += kAttWarps * 128) {
+        float4 sum = *reinterpret_cast<const float4 *>(part_o + i);
+#pragma unroll
+        for (int k = 1; k < kAttWarps; ++k) {
+            const float4 x = *reinterpret_cast<const float4 *>(part_o + k * kRows * D + i);
+            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+        }
+        *reinterpret_cast<float4 *>(part_o + i) = sum;
     }
 
     // the CTAs' results are joined, a share of the numbers by each CTA
@@ -525,27 +586,30 @@ __global__ void __launch_bounds__(kAttWarps * 32) kv_attention_kernel(AttentionA
     else __syncthreads();
     const int part = split / a.cluster;
     float *ws = a.parts > 1 ? a.workspace + (unit * a.parts + part) * (kRows * (D + 2)) : nullptr;
-    for (int i = (int)rank * kAttWarps * 32 + threadIdx.x; i < kRows * D; i += a.cluster * kAttWarps * 32) {
+    for (int i = ((int)rank * kAttWarps * 32 + threadIdx.x) * 4; i < live * D; i += a.cluster * kAttWarps * 128) {
         const int row = i / D, d = i % D;
-        if (row0 + row > last_row || d >= a.dim) continue;
-        float peak = -INFINITY, total = 0.0f, sum = 0.0f;
+        if (d >= dim) continue;
+        float peak = -INFINITY, total = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (a.cluster == 1) {
-            peak = all_m[row], total = all_l[row], sum = part_o[i];
+            peak = all_m[row], total = all_l[row], sum = *reinterpret_cast<const float4 *>(part_o + i);
         } else {
             for (int k = 0; k < a.cluster; ++k) peak = fmaxf(peak, remote_load(all_m + row, k));
             for (int k = 0; k < a.cluster; ++k) {
-                const float x = remote_load(all_m + row, k), turn = x == -INFINITY ? 1.0f : exp2f(x - peak);
+                const float x = remote_load(all_m + row, k), turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
+                const float4 y = remote_load4(part_o + i, k);
                 total += turn * remote_load(all_l + row, k);
-                sum += turn * remote_load(part_o + i, k);
+                sum.x += turn * y.x, sum.y += turn * y.y, sum.z += turn * y.z, sum.w += turn * y.w;
             }
         }
         if (a.parts > 1) {
-            ws[i] = sum;
+            *reinterpret_cast<float4 *>(ws + i) = sum;
             if (d == 0) ws[kRows * D + row] = peak, ws[kRows * D + kRows + row] = total;
         } else {
             const int64_t at = row0 + row, query = at / a.group, hq = h * a.group + at % a.group;
-            ((T *)a.out)[((b * a.queries + query) * (a.kv_heads * a.group) + hq) * a.dim + d] =
-                df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
+            const float turn = total == 0.0f ? 0.0f : 1.0f / total;
+            sum.x *= turn, sum.y *= turn, sum.z *= turn, sum.w *= turn;
+            store4((T *)a.out + ((b * a.queries + query) * (a.kv_heads * a.group) + hq) * dim + d, sum);
         }
     }
     if (a.cluster > 1) cluster_barrier();               // nobody leaves while its memory is read
@@ -563,7 +627,7 @@ template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_att
     for (int k = 0; k < a.parts; ++k) peak = fmaxf(peak, ws[k * (kRows * (D + 2)) + kRows * D + row]);
     for (int k = 0; k < a.parts; ++k) {
         const float *part = ws + k * (kRows * (D + 2));
-        const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2f(x - peak);
+        const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
         total += turn * part[kRows * D + kRows + row];
         sum += turn * part[row * D + d];
     }
@@ -596,12 +660,12 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
     return d;
 }
 
-template <int D, int NT, int FMT, typename T>
+template <int D, int NT, int FMT, bool EXACT, typename T>
 cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStream_t stream)
 {
     constexpr int kRows = NT * 8;
     constexpr size_t kShared = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
-    auto kernel = kv_attention_kernel<D, NT, FMT, T>;
+    auto kernel = kv_attention_kernel<D, NT, FMT, EXACT, T>;
     if (kShared > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
         if (e != cudaSuccess) return e;
@@ -625,10 +689,14 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStre
 
 template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, cudaStream_t stream)
 {
-#define DF11_ATTENTION(D, NT)                                                                     \
-    if (d.width == D && d.tiles_n == NT)                                                          \
-        return format == DF11_KV_INT8 ? launch_attention<D, NT, DF11_KV_INT8, T>(a, d, stream)    \
-                                      : launch_attention<D, NT, DF11_KV_E4M3, T>(a, d, stream);
+#define DF11_ATTENTION(D, NT)                                                                             \
+    if (d.width == D && d.tiles_n == NT) {                                                                \
+        if (format == DF11_KV_INT8)                                                                       \
+            return a.dim == D ? launch_attention<D, NT, DF11_KV_INT8, true, T>(a, d, stream)              \
+                              : launch_attention<D, NT, DF11_KV_INT8, false, T>(a, d, stream);            \
+        return a.dim == D ? launch_attention<D, NT, DF11_KV_E4M3, true, T>(a, d, stream)                  \
+                          : launch_attention<D, NT, DF11_KV_E4M3, false, T>(a, d, stream);                \
+    }
     DF11_ATTENTION(64, 1)
     DF11_ATTENTION(64, 2)
     DF11_ATTENTION(128, 1)

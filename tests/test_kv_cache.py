@@ -8,6 +8,10 @@ Codes and scales are compared bit for bit.  The bound for attention, per output 
                          the other, each step rounded by at most 2^-22 of the running sum (truncating adders included)
   + A (n/16 + 64) 2^-22  the sums over n slots, 16 of which meet in one step, and the joins of parts
 plus 2^-24 of the row's largest query entry per product for entries that fp16 holds as subnormals.
+The int8 kernel multiplies code + 128 and takes 128 times the other operand's sum off again, so what its sums round
+are steps of size |code| + 128: in the two terms with 2^-22, |k| and |v| are |k| + 128 k_scale and |v| + 128 v_scale.
+(With one slot seen the result is the value itself and A = |v|; a code of 1 then carries 129 2^-22 = 2^-15 of itself,
+which is beside the 2^-11 of the weight but not nothing.)
 """
 import numpy as np
 import pytest
@@ -172,11 +176,12 @@ def reference_attention(q, cache, lengths, first, scale, window):
                 v = vc[b, g, low:high + 1] * vs[b, g, low:high + 1, None]
                 p = torch.softmax(k @ q[b, h, i] * scale, 0)
                 out[b, i, h] = p @ v
-                magnitude = p @ v.abs()
-                score = float((k.abs() @ q[b, h, i].abs()).max()) * abs(scale)
+                magnitude, shift = p @ v.abs(), 128 * (cache[0].dtype == torch.int8)
+                stepped = magnitude + shift * (p @ vs[b, g, low:high + 1])
+                score = float(((k.abs() + shift * ks[b, g, low:high + 1, None]) @ q[b, h, i].abs()).max()) * abs(scale)
                 small = dim * 2.0 ** -24 * float(q[b, h, i].abs().max() * k.abs().max()) * abs(scale)
                 ds = (dim + 8) * 2.0 ** -22 * score + small
-                bound[b, i, h] = magnitude * (2.0 ** -11 + 2 * ds + ((high - low + 1) / 16 + 64) * 2.0 ** -22)
+                bound[b, i, h] = magnitude * (2.0 ** -11 + 2 * ds) + stepped * ((high - low + 1) / 16 + 64) * 2.0 ** -22
     return out, bound
 
 
