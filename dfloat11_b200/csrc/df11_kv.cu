@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const uint8_t *k_codes, co
 // distributed shared memory, and, for long caches with few heads, among several such clusters
 // whose results a second kernel joins in a fixed order.
 constexpr int kAttWarps = 4;
+template <int D> constexpr int kAttStages = D == 64 ? 4 : 3;       // tiles of 16 slots under way per warp, one in use
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -180,21 +181,24 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b)
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 
-template <int BYTES> struct Bytes;
-template <> struct Bytes<8> {
-    uint32_t w[2];
-    __device__ __forceinline__ void load(const uint8_t *p)
+// BYTES bytes of one thread: copied to its own place in shared memory ahead of time, read when needed.
+template <int BYTES> struct Bytes {
+    uint32_t w[BYTES / 4];
+    static __device__ __forceinline__ void fetch(uint8_t *to, const uint8_t *from)
     {
-        const uint2 x = __ldg(reinterpret_cast<const uint2 *>(p));
-        w[0] = x.x, w[1] = x.y;
+        const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+        if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
     }
-};
-template <> struct Bytes<16> {
-    uint32_t w[4];
-    __device__ __forceinline__ void load(const uint8_t *p)
+    __device__ __forceinline__ void load(const uint8_t *from)
     {
-        const uint4 x = __ldg(reinterpret_cast<const uint4 *>(p));
-        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+        if (BYTES == 16) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(from);
+            w[0] = x.x, w[1] = x.y, w[BYTES / 4 - 2] = x.z, w[BYTES / 4 - 1] = x.w;
+        } else {
+            const uint2 x = *reinterpret_cast<const uint2 *>(from);
+            w[0] = x.x, w[BYTES / 4 - 1] = x.y;
+        }
     }
 };
 
@@ -207,8 +211,9 @@ struct AttentionArgs {
     int length_per, first_per;
     void *out;
     float *workspace;                   // [unit][parts][rows * (D + 2)] where parts > 1
-    int kv_heads, group, dim, window, row_groups, cluster, parts, q_aligned;
-    int64_t queries, max_slots;
+    uint32_t kv_heads, group, queries, row_groups, cluster, parts;
+    int dim, window, q_aligned;
+    int64_t max_slots;
     float scale;
 };
 
@@ -216,9 +221,9 @@ struct AttentionArgs {
 struct Sight {
     int64_t low, high;
 };
-__device__ __forceinline__ Sight sight_of(const AttentionArgs &a, int64_t length, int64_t first, int64_t query)
+__device__ __forceinline__ Sight sight_of(const AttentionArgs &a, int64_t length, int64_t first, uint32_t query)
 {
-    const int64_t place = length - a.queries + query;
+    const int64_t place = length - (int64_t)a.queries + query;
     int64_t low = first;
     if (a.window > 0 && place - a.window + 1 > low) low = place - a.window + 1;
     return {low, place < a.max_slots ? place : a.max_slots - 1};
@@ -269,14 +274,15 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float4 x)
 // EXACT: head_dim is D; otherwise it is smaller, and what is loaded beyond it is some other chunk of the
 // same row that meets a zero of the query or ends in a result that nobody reads.
 template <int D, int NT, int FMT, bool EXACT, typename T>
-__global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 128 ? 3 : 2) kv_attention_kernel(AttentionArgs a)
+__global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 5 - NT : 2) kv_attention_kernel(AttentionArgs a)
 {
     constexpr int kRows = NT * 8;
     constexpr int kKeyChunks = D / 64;                      // 16-byte chunks of a key row per thread
     constexpr int kValBytes = D >= 128 ? 16 : D / 8;        // consecutive bytes of a value row per thread
     constexpr int kValChunks = D / 8 / kValBytes;
     constexpr int kBlocks = D / 16;                         // fragments of 16 dimensions
-    extern __shared__ float shared[];
+    constexpr int kStages = kAttStages<D>, kStageBytes = 32 * D + 128;
+    extern __shared__ __align__(16) float shared[];
     float *part_o = shared;                                 // [warps][rows][D]
     float *part_m = part_o + kAttWarps * kRows * D;         // [warps][rows]
     float *part_l = part_m + kAttWarps * kRows;
@@ -284,13 +290,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
     float *all_l = all_m + kRows;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-    const int splits = a.cluster * a.parts;
-    const int64_t unit = blockIdx.x / splits;
-    const int split = blockIdx.x % splits;
-    const int64_t head = unit / a.row_groups, b = head / a.kv_heads;
-    const int h = (int)(head % a.kv_heads);
-    const int64_t row0 = unit % a.row_groups * kRows, rows = (int64_t)a.group * a.queries;
-    const int64_t last_row = min(row0 + kRows, rows) - 1;
+    const uint32_t splits = a.cluster * a.parts, unit = blockIdx.x / splits, split = blockIdx.x % splits;
+    const uint32_t head = unit / a.row_groups, b = head / a.kv_heads, h = head % a.kv_heads;
+    const uint32_t row0 = unit % a.row_groups * kRows, rows = a.group * a.queries, last_row = min(row0 + kRows, rows) - 1;
 
     // the query fragments, in the order in which the key bytes lie
     uint32_t qf[NT][D / 16][2];
@@ -298,8 +300,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
     float offset[NT][2] = {};                               // what the sum starts from: - 128 sum(q) in the codes' unit
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int64_t row = min(row0 + nt * 8 + r, rows - 1);
-        const T *x = (const T *)a.q + b * a.qs.b + (h * a.group + row % a.group) * a.qs.h + row / a.group * a.qs.t;
+        const uint32_t row = min(row0 + nt * 8 + r, last_row), query = row / a.group;
+        const T *x = (const T *)a.q + b * a.qs.b + (h * a.group + (row - query * a.group)) * a.qs.h + query * a.qs.t;
         float peak = 0.0f;
         uint32_t raw[D / 16][2];
 #pragma unroll
@@ -369,14 +371,14 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const Sight s = sight_of(a, length, start, min(row0 + nt * 8 + 2 * c + i, rows - 1) / a.group);
+            const Sight s = sight_of(a, length, start, min(row0 + nt * 8 + 2 * c + i, last_row) / a.group);
             col_low[nt][i] = (int)min(s.low - low, n);
             col_high[nt][i] = (int)max(s.high - low, (int64_t)-1);
         }
 
-    const int64_t tiles = (n + 15) / 16;
-    const int begin = (int)(tiles * split / splits), end = (int)(tiles * (split + 1) / splits);
-    const int64_t cell0 = head * a.max_slots + low;
+    const uint32_t tiles = (uint32_t)((n + 15) / 16), share = tiles / splits, extra = tiles - share * splits;
+    const int begin = (int)(share * split + min(split, extra)), end = begin + (int)(share + (split < extra));
+    const int64_t cell0 = (int64_t)head * a.max_slots + low;
 
     float o[kBlocks][NT][4] = {}, o128[NT][4] = {};         // o128: 128 times the sum of the weights, in the codes' unit
     // running maximum, sum, factor on weight * scale, and the largest weight * scale when it was set;
@@ -385,9 +387,6 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, f[nt][0] = f[nt][1] = 0x1p126f;
 
-    Bytes<16> kx[2][kKeyChunks];
-    Bytes<kValBytes> vx[4][kValChunks];
-    float ks[2], vs[2];
     const int dim = EXACT ? D : a.dim;
     // a thread's places in a tile of 16 slots: key rows r and r + 8, value rows 2c, 2c + 1, 2c + 8, 2c + 9
     int key_at[kKeyChunks], value_at[kValChunks];
@@ -397,36 +396,71 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
     for (int j = 0; j < kValChunks; ++j) value_at[j] = EXACT ? j * 8 * kValBytes : min((j * 8 + r) * kValBytes, dim - kValBytes);
     const uint8_t *const key_base = a.k_codes + cell0 * dim + (EXACT ? c * 16 : 0);
     const uint8_t *const value_base = a.v_codes + cell0 * dim + (EXACT ? r * kValBytes : 0);
-    const float *const key_scales = a.k_scales + cell0, *const value_scales = a.v_scales + cell0;
-    // Past the last slot the last one is loaded again: its weight is 0 there, and whatever lies in the
+    // A warp's tiles come through a ring in shared memory, in which every thread has its own bytes; only
+    // the scales (of keys r and r + 8, of values r and r + 8) are fetched for one another.
+    // Past the last slot the last one is fetched again: its weight is 0 there, and whatever lies in the
     // cache behind it (a NaN, say) does not reach a product.
-    auto load_keys = [&](int tile) {
-        const uint8_t *p = key_base + (int64_t)tile * 16 * dim;
+    uint8_t *const ring = reinterpret_cast<uint8_t *>(shared) + warp * (kStages * kStageBytes);
+    const float *const scale_base = (c < 2 ? a.k_scales : a.v_scales) + cell0;
+    auto fetch = [&](int tile, uint8_t *stage) {
         const int s0 = tile * 16, left = count - 1 - s0;
-        const int r0 = left < 15 ? min(r, left) : r, r1 = left < 15 ? min(r + 8, left) : r + 8;
-        ks[0] = __ldg(key_scales + s0 + r0), ks[1] = __ldg(key_scales + s0 + r1);
-        vs[0] = __ldg(value_scales + s0 + r0), vs[1] = __ldg(value_scales + s0 + r1);
+        const uint8_t *const kp = key_base + (int64_t)s0 * dim, *const vp = value_base + (int64_t)s0 * dim;
+        const int rs = r + 8 * (c & 1);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(stage + 32 * D + lane * 4)),
+                     "l"(scale_base + s0 + min(rs, left))
+                     : "memory");
+        if (left >= 15) {
 #pragma unroll
-        for (int j = 0; j < kKeyChunks; ++j) {
-            kx[0][j].load(p + r0 * dim + key_at[j]);
-            kx[1][j].load(p + r1 * dim + key_at[j]);
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < kKeyChunks; ++j)
+                    Bytes<16>::fetch(stage + ((i * kKeyChunks + j) * 32 + lane) * 16, kp + r * dim + 8 * i * dim + key_at[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kValChunks; ++j)
+                    Bytes<kValBytes>::fetch(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes,
+                                            vp + 2 * c * dim + ((i & 1) + 8 * (i >> 1)) * dim + value_at[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < kKeyChunks; ++j)
+                    Bytes<16>::fetch(stage + ((i * kKeyChunks + j) * 32 + lane) * 16, kp + min(r + 8 * i, left) * dim + key_at[j]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < kValChunks; ++j)
+                    Bytes<kValBytes>::fetch(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes,
+                                            vp + min(2 * c + (i & 1) + 8 * (i >> 1), left) * dim + value_at[j]);
         }
     };
-    auto load_values = [&](int tile) {
-        const uint8_t *p = value_base + (int64_t)tile * 16 * dim;
-        const int left = count - 1 - tile * 16;
+    int ahead = begin + warp;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int at = 2 * c + (i & 1) + 8 * (i >> 1), row = left < 15 ? min(at, left) : at;
-#pragma unroll
-            for (int j = 0; j < kValChunks; ++j) vx[i][j].load(p + row * dim + value_at[j]);
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (ahead < end) fetch(ahead, ring + i * kStageBytes);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += kAttWarps;
+    }
+    int at_stage = 0;
+    for (int tile = begin + warp; tile < end; tile += kAttWarps) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        const uint8_t *const stage = ring + at_stage * kStageBytes;
+        {
+            const int to = at_stage == 0 ? kStages - 1 : at_stage - 1;      // read in the step before
+            if (ahead < end) fetch(ahead, ring + to * kStageBytes);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ahead += kAttWarps;
+            at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
         }
-    };
-
-    int tile = begin + warp;
-    if (tile < end) load_keys(tile), load_values(tile);
-    for (; tile < end; tile += kAttWarps) {
-        const bool more = tile + kAttWarps < end;
+        const float4 scales = *reinterpret_cast<const float4 *>(stage + 32 * D + r * 16);
+        const float key_scale[2] = {scales.x, scales.y}, value_scale[2] = {scales.z, scales.w};
+        Bytes<16> kx[2][kKeyChunks];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < kKeyChunks; ++j) kx[i][j].load(stage + ((i * kKeyChunks + j) * 32 + lane) * 16);
         float s[NT][4], s2[NT][4] = {};                     // two chains of sums: a product waits for the last of its chain
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][2] = offset[nt][0], s[nt][1] = s[nt][3] = offset[nt][1];
@@ -440,8 +474,11 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma_16x8x16(w & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][j * 4 + w][0], qf[nt][j * 4 + w][1]);
             }
-        const float key_scale[2] = {ks[0], ks[1]}, value_scale[2] = {vs[0], vs[1]};
-        if (more) load_keys(tile + kAttWarps);
+        Bytes<kValBytes> vx[4][kValChunks];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < kValChunks; ++j) vx[i][j].load(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes);
 
         const int s0 = tile * 16;
         const bool whole = s0 >= inner_low && s0 + 15 <= inner_high;    // every row sees every slot
@@ -524,8 +561,9 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[k][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                 }
-        if (more) load_values(tile + kAttWarps);
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();                                        // the ring's memory is used for the results
 
     // the warps' results are joined
 #pragma unroll
@@ -584,8 +622,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
     const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0;
     if (a.cluster > 1) cluster_barrier();
     else __syncthreads();
-    const int part = split / a.cluster;
-    float *ws = a.parts > 1 ? a.workspace + (unit * a.parts + part) * (kRows * (D + 2)) : nullptr;
+    float *ws = a.parts > 1 ? a.workspace + (int64_t)(blockIdx.x / a.cluster) * (kRows * (D + 2)) : nullptr;
     for (int i = ((int)rank * kAttWarps * 32 + threadIdx.x) * 4; i < live * D; i += a.cluster * kAttWarps * 128) {
         const int row = i / D, d = i % D;
         if (d >= dim) continue;
@@ -594,8 +631,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
         if (a.cluster == 1) {
             peak = all_m[row], total = all_l[row], sum = *reinterpret_cast<const float4 *>(part_o + i);
         } else {
-            for (int k = 0; k < a.cluster; ++k) peak = fmaxf(peak, remote_load(all_m + row, k));
-            for (int k = 0; k < a.cluster; ++k) {
+            for (uint32_t k = 0; k < a.cluster; ++k) peak = fmaxf(peak, remote_load(all_m + row, k));
+            for (uint32_t k = 0; k < a.cluster; ++k) {
                 const float x = remote_load(all_m + row, k), turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
                 const float4 y = remote_load4(part_o + i, k);
                 total += turn * remote_load(all_l + row, k);
@@ -606,10 +643,10 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
             *reinterpret_cast<float4 *>(ws + i) = sum;
             if (d == 0) ws[kRows * D + row] = peak, ws[kRows * D + kRows + row] = total;
         } else {
-            const int64_t at = row0 + row, query = at / a.group, hq = h * a.group + at % a.group;
+            const uint32_t at = row0 + row, query = at / a.group, hq = h * a.group + (at - query * a.group);
             const float turn = total == 0.0f ? 0.0f : 1.0f / total;
             sum.x *= turn, sum.y *= turn, sum.z *= turn, sum.w *= turn;
-            store4((T *)a.out + ((b * a.queries + query) * (a.kv_heads * a.group) + hq) * dim + d, sum);
+            store4((T *)a.out + (((int64_t)b * a.queries + query) * (a.kv_heads * a.group) + hq) * dim + d, sum);
         }
     }
     if (a.cluster > 1) cluster_barrier();               // nobody leaves while its memory is read
@@ -619,20 +656,20 @@ __global__ void __launch_bounds__(kAttWarps * 32, D * NT <= 64 ? 4 : D * NT <= 1
 template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_attention_join_kernel(AttentionArgs a)
 {
     constexpr int kRows = NT * 8;
-    const int64_t rows = (int64_t)a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
+    const uint32_t rows = a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
     const int row = (int)(at % kRows), d = threadIdx.x;
-    const float *ws = a.workspace + (head * a.row_groups + at / kRows) * a.parts * (kRows * (D + 2));
+    const float *ws = a.workspace + (int64_t)(head * a.row_groups + at / kRows) * a.parts * (kRows * (D + 2));
     if (d >= a.dim) return;
     float peak = -INFINITY, total = 0.0f, sum = 0.0f;
-    for (int k = 0; k < a.parts; ++k) peak = fmaxf(peak, ws[k * (kRows * (D + 2)) + kRows * D + row]);
-    for (int k = 0; k < a.parts; ++k) {
+    for (uint32_t k = 0; k < a.parts; ++k) peak = fmaxf(peak, ws[k * (kRows * (D + 2)) + kRows * D + row]);
+    for (uint32_t k = 0; k < a.parts; ++k) {
         const float *part = ws + k * (kRows * (D + 2));
         const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
         total += turn * part[kRows * D + kRows + row];
         sum += turn * part[row * D + d];
     }
-    const int64_t hq = head % a.kv_heads * a.group + at % a.group;
-    ((T *)a.out)[((b * a.queries + at / a.group) * (a.kv_heads * a.group) + hq) * a.dim + d] =
+    const uint32_t hq = head % a.kv_heads * a.group + at % a.group;
+    ((T *)a.out)[(((int64_t)b * a.queries + at / a.group) * (a.kv_heads * a.group) + hq) * a.dim + d] =
         df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
 }
 
@@ -664,7 +701,8 @@ template <int D, int NT, int FMT, bool EXACT, typename T>
 cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStream_t stream)
 {
     constexpr int kRows = NT * 8;
-    constexpr size_t kShared = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
+    constexpr size_t kJoin = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
+    constexpr size_t kRing = (size_t)kAttWarps * kAttStages<D> * (32 * D + 128), kShared = kRing > kJoin ? kRing : kJoin;
     auto kernel = kv_attention_kernel<D, NT, FMT, EXACT, T>;
     if (kShared > 48 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
@@ -683,7 +721,7 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStre
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
     if (e != cudaSuccess || d.parts == 1) return e;
     const int64_t heads = d.units / d.row_groups;
-    kv_attention_join_kernel<D, NT, T><<<(unsigned)(heads * a.group * a.queries), D, 0, stream>>>(a);
+    kv_attention_join_kernel<D, NT, T><<<(unsigned)(heads * ((int64_t)a.group * a.queries)), D, 0, stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -841,9 +879,9 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     a.lengths = (const int64_t *)lengths, a.length_per = n_lengths > 1;
     a.first = (const int64_t *)first, a.first_per = n_first > 1;
     a.out = out, a.workspace = (float *)workspace;
-    a.kv_heads = kv_heads, a.group = heads / kv_heads, a.dim = head_dim, a.window = window;
-    a.row_groups = (int)d.row_groups, a.cluster = d.cluster, a.parts = d.parts;
-    a.queries = queries, a.max_slots = max_slots, a.scale = scale;
+    a.kv_heads = (uint32_t)kv_heads, a.group = (uint32_t)(heads / kv_heads), a.dim = head_dim, a.window = window;
+    a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster, a.parts = (uint32_t)d.parts;
+    a.queries = (uint32_t)queries, a.max_slots = max_slots, a.scale = scale;
     const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, (cudaStream_t)stream)
                                                          : launch_attention<__half>(a, d, format, (cudaStream_t)stream);
     if (e != cudaSuccess) return df11_fail(DF11_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
