@@ -127,9 +127,10 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const uint8_t *k_codes, co
 // fp16 holds exactly from there down to 2^-24; smaller entries are rounded to multiples of 2^-24 of that.
 // Sums, maxima and denominators are fp32.
 //
-// The slots of a sequence are divided among `cluster` CTAs that join their results through
-// distributed shared memory, and, for long caches with few heads, among several such clusters
-// whose results a second kernel joins in a fixed order.
+// Small calls: the slots of a sequence are divided among a cluster of CTAs that join their results
+// through distributed shared memory, in one launch.  Large ones: the tiles of all sequences and heads are
+// cut into equal lengths, one per resident CTA, so that sequences of any lengths keep every SM busy
+// to the end; a second kernel joins, in a fixed order, what was cut.
 constexpr int kAttWarps = 4;
 template <int D> constexpr int kAttStages = D == 64 ? 4 : 3;       // tiles of 16 slots under way per warp, one in use
 constexpr float kLog2e = 1.4426950408889634f;
@@ -210,8 +211,8 @@ struct AttentionArgs {
     const int64_t *lengths, *first;
     int length_per, first_per;
     void *out;
-    float *workspace;                   // [unit][parts][rows * (D + 2)] where parts > 1
-    uint32_t kv_heads, group, queries, row_groups, cluster, parts;
+    float *workspace;                   // shared out: two results of rows * (D + 2) numbers per CTA
+    uint32_t batch, kv_heads, group, queries, row_groups, cluster;
     int dim, window, q_aligned;
     int64_t max_slots;
     float scale;
@@ -228,6 +229,55 @@ __device__ __forceinline__ Sight sight_of(const AttentionArgs &a, int64_t length
     if (a.window > 0 && place - a.window + 1 > low) low = place - a.window + 1;
     return {low, place < a.max_slots ? place : a.max_slots - 1};
 }
+
+// Shared out: the slots of all sequences in tiles of 16, one row of tiles per key head and row group, cut
+// into equal lengths.  Everything here follows from the sequences' lengths, so every CTA finds its own
+// share, and the joining kernel every share, without asking anyone.
+struct Sequence {
+    uint32_t index, tiles, before;      // before: tiles per head of the sequences ahead of it
+};
+
+__device__ __forceinline__ uint32_t tiles_of(const AttentionArgs &a, uint32_t b)
+{
+    if (b >= a.batch) return 0;
+    const int64_t length = clamped_length(a.lengths[a.length_per ? b : 0]);
+    const int64_t start = a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
+    const int64_t n = sight_of(a, length, start, a.queries - 1).high - sight_of(a, length, start, 0).low + 1;
+    return n > 0 ? (uint32_t)((n + 15) / 16) : 0;
+}
+
+// The whole warp: tiles per head of all sequences.
+__device__ __forceinline__ uint32_t all_tiles(const AttentionArgs &a)
+{
+    uint32_t sum = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 32) sum += __reduce_add_sync(0xffffffffu, tiles_of(a, b0 + (threadIdx.x & 31)));
+    return sum;
+}
+
+// The whole warp: the sequence that holds tile `at` (of all heads' tiles), or, by index, sequence `want`.
+template <bool BY_INDEX> __device__ __forceinline__ Sequence find_sequence(const AttentionArgs &a, uint32_t want)
+{
+    const uint32_t lane = threadIdx.x & 31, heads = a.kv_heads * a.row_groups;
+    uint32_t before = 0;
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 32) {
+        const uint32_t mine = tiles_of(a, b0 + lane);
+        uint32_t sum = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= (uint32_t)d) sum += x;
+        }
+        const uint32_t hit = __ballot_sync(0xffffffffu, BY_INDEX ? b0 + lane == want : (before + sum) * heads > want);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            return {b0 + at, __shfl_sync(0xffffffffu, mine, at), before + __shfl_sync(0xffffffffu, sum - mine, at)};
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return {a.batch, 0, before};
+}
+
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t ctas) { return max((total + ctas - 1) / ctas, 8u); }
 
 __device__ __forceinline__ uint32_t cluster_rank()
 {
@@ -273,8 +323,10 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float4 x)
 // One CTA: up to NT * 8 query rows of one key head, and its share of the slots they see.
 // EXACT: head_dim is D; otherwise it is smaller, and what is loaded beyond it is some other chunk of the
 // same row that meets a zero of the query or ends in a result that nobody reads.
-template <int D, int NT, int FMT, bool EXACT, typename T>
-__global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 5 - NT : 2) kv_attention_kernel(AttentionArgs a)
+// SHARED: tiles [first_tile, last_tile) of the sequence, the result to `ws` if they are not all of them;
+// otherwise the CTAs of a cluster take equal parts.
+template <int D, int NT, int FMT, bool EXACT, bool SHARED, typename T>
+__device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, uint32_t first_tile, uint32_t last_tile, float *ws)
 {
     constexpr int kRows = NT * 8;
     constexpr int kKeyChunks = D / 64;                      // 16-byte chunks of a key row per thread
@@ -290,7 +342,6 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
     float *all_l = all_m + kRows;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
-    const uint32_t splits = a.cluster * a.parts, unit = blockIdx.x / splits, split = blockIdx.x % splits;
     const uint32_t head = unit / a.row_groups, b = head / a.kv_heads, h = head % a.kv_heads;
     const uint32_t row0 = unit % a.row_groups * kRows, rows = a.group * a.queries, last_row = min(row0 + kRows, rows) - 1;
 
@@ -363,7 +414,8 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
     const int64_t length = clamped_length(a.lengths[a.length_per ? b : 0]);
     const int64_t start = a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
     const Sight top = sight_of(a, length, start, row0 / a.group), bottom = sight_of(a, length, start, last_row / a.group);
-    const int64_t low = top.low, n = max(bottom.high - low + 1, (int64_t)0);
+    const int64_t low = SHARED ? sight_of(a, length, start, 0).low : top.low;
+    const int64_t n = max((SHARED ? sight_of(a, length, start, a.queries - 1).high : bottom.high) - low + 1, (int64_t)0);
     const int inner_low = (int)min(bottom.low - low, n), inner_high = (int)max(top.high - low, (int64_t)-1);
     const int count = (int)n;
     int col_low[NT][2], col_high[NT][2];                    // relative to `low`
@@ -376,8 +428,12 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
             col_high[nt][i] = (int)max(s.high - low, (int64_t)-1);
         }
 
-    const uint32_t tiles = (uint32_t)((n + 15) / 16), share = tiles / splits, extra = tiles - share * splits;
-    const int begin = (int)(share * split + min(split, extra)), end = begin + (int)(share + (split < extra));
+    const uint32_t rank = !SHARED && a.cluster > 1 ? cluster_rank() : 0;
+    if (!SHARED) {
+        const uint32_t tiles = (uint32_t)((n + 15) / 16), share = tiles / a.cluster, extra = tiles - share * a.cluster;
+        first_tile = share * rank + min(rank, extra), last_tile = first_tile + share + (rank < extra);
+    }
+    const int begin = (int)first_tile, end = min((int)last_tile, (int)((n + 15) / 16));
     const int64_t cell0 = (int64_t)head * a.max_slots + low;
 
     float o[kBlocks][NT][4] = {}, o128[NT][4] = {};         // o128: 128 times the sum of the weights, in the codes' unit
@@ -618,17 +674,15 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
         *reinterpret_cast<float4 *>(part_o + i) = sum;
     }
 
-    // the CTAs' results are joined, a share of the numbers by each CTA
-    const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0;
-    if (a.cluster > 1) cluster_barrier();
+    // the results of a cluster's CTAs are joined, a share of the numbers by each
+    if (!SHARED && a.cluster > 1) cluster_barrier();
     else __syncthreads();
-    float *ws = a.parts > 1 ? a.workspace + (int64_t)(blockIdx.x / a.cluster) * (kRows * (D + 2)) : nullptr;
-    for (int i = ((int)rank * kAttWarps * 32 + threadIdx.x) * 4; i < live * D; i += a.cluster * kAttWarps * 128) {
+    for (int i = ((int)rank * kAttWarps * 32 + threadIdx.x) * 4; i < live * D; i += (SHARED ? 1 : a.cluster) * kAttWarps * 128) {
         const int row = i / D, d = i % D;
         if (d >= dim) continue;
         float peak = -INFINITY, total = 0.0f;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (a.cluster == 1) {
+        if (SHARED || a.cluster == 1) {
             peak = all_m[row], total = all_l[row], sum = *reinterpret_cast<const float4 *>(part_o + i);
         } else {
             for (uint32_t k = 0; k < a.cluster; ++k) peak = fmaxf(peak, remote_load(all_m + row, k));
@@ -639,7 +693,7 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
                 sum.x += turn * y.x, sum.y += turn * y.y, sum.z += turn * y.z, sum.w += turn * y.w;
             }
         }
-        if (a.parts > 1) {
+        if (SHARED && ws) {
             *reinterpret_cast<float4 *>(ws + i) = sum;
             if (d == 0) ws[kRows * D + row] = peak, ws[kRows * D + kRows + row] = total;
         } else {
@@ -649,35 +703,84 @@ __global__ void __launch_bounds__(kAttWarps * 32, D == 128 ? 4 / NT : D == 64 ? 
             store4((T *)a.out + (((int64_t)b * a.queries + query) * (a.kv_heads * a.group) + hq) * dim + d, sum);
         }
     }
-    if (a.cluster > 1) cluster_barrier();               // nobody leaves while its memory is read
+    if (!SHARED && a.cluster > 1) cluster_barrier();    // nobody leaves while its memory is read
+    if (SHARED) __syncthreads();                        // the next stretch fills the same memory
 }
 
-// Joins the clusters' results: one CTA per query row.
-template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_attention_join_kernel(AttentionArgs a)
+template <int D, int NT> constexpr int kAttCtas = D == 128 ? 4 / NT : D == 64 ? 5 - NT : 2;   // per SM, by registers and memory
+
+template <int D, int NT, int FMT, bool EXACT, typename T>
+__global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attention_kernel(AttentionArgs a)
+{
+    attend<D, NT, FMT, EXACT, false, T>(a, blockIdx.x / a.cluster, 0, 0, nullptr);
+}
+
+template <int D, int NT, int FMT, bool EXACT, typename T>
+__global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attention_shared_kernel(AttentionArgs a)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the joining kernel may take its places
+    const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, gridDim.x);
+    if ((uint64_t)share * blockIdx.x >= total) return;
+    uint32_t at = share * blockIdx.x;
+    const uint32_t end = min(at + share, total);
+    Sequence s = find_sequence<false>(a, at);
+    bool front = true;
+    while (at < end && s.tiles) {
+        const uint32_t inside = at - s.before * heads, unit = inside / s.tiles, first = inside - unit * s.tiles;
+        const uint32_t last = min(s.tiles, first + (end - at));
+        float *ws = first == 0 && last == s.tiles ? nullptr
+                  : a.workspace + ((int64_t)blockIdx.x * 2 + !front) * (NT * 8 * (D + 2));
+        attend<D, NT, FMT, EXACT, true, T>(a, s.index * heads + unit, first, last, ws);
+        at += last - first;
+        front = false;
+        if (at < end && unit + 1 == heads && last == s.tiles) {
+            s.before += s.tiles;
+            do s.tiles = tiles_of(a, ++s.index); while (s.tiles == 0 && s.index < a.batch);
+        }
+    }
+}
+
+// Joins the shares of a sequence that was cut, and writes the zeros of one that has no slots: one CTA
+// per query row.
+template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_attention_join_kernel(AttentionArgs a, uint32_t ctas)
 {
     constexpr int kRows = NT * 8;
     const uint32_t rows = a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
+    const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, ctas);
+    const Sequence s = find_sequence<true>(a, b);
+    const uint32_t from = s.before * heads + (head % a.kv_heads * a.row_groups + at / kRows) * s.tiles;
+    const uint32_t j0 = from / share, j1 = s.tiles ? (from + s.tiles - 1) / share : j0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");                  // the shares are written
     const int row = (int)(at % kRows), d = threadIdx.x;
-    const float *ws = a.workspace + (int64_t)(head * a.row_groups + at / kRows) * a.parts * (kRows * (D + 2));
-    if (d >= a.dim) return;
-    float peak = -INFINITY, total = 0.0f, sum = 0.0f;
-    for (uint32_t k = 0; k < a.parts; ++k) peak = fmaxf(peak, ws[k * (kRows * (D + 2)) + kRows * D + row]);
-    for (uint32_t k = 0; k < a.parts; ++k) {
-        const float *part = ws + k * (kRows * (D + 2));
-        const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
-        total += turn * part[kRows * D + kRows + row];
-        sum += turn * part[row * D + d];
+    if (d >= a.dim || (s.tiles && j0 == j1)) return;
+    const float *const first = a.workspace + ((int64_t)j0 * 2 + (j0 * share != from)) * (kRows * (D + 2));
+    float peak = -INFINITY, sum = 0.0f, l = 0.0f;
+    if (s.tiles) {
+        for (uint32_t j = j0; j <= j1; ++j) {
+            const float *part = j == j0 ? first : a.workspace + (int64_t)j * 2 * (kRows * (D + 2));
+            peak = fmaxf(peak, part[kRows * D + row]);
+        }
+        for (uint32_t j = j0; j <= j1; ++j) {
+            const float *part = j == j0 ? first : a.workspace + (int64_t)j * 2 * (kRows * (D + 2));
+            const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
+            l += turn * part[kRows * D + kRows + row];
+            sum += turn * part[row * D + d];
+        }
     }
-    const uint32_t hq = head % a.kv_heads * a.group + at % a.group;
-    ((T *)a.out)[(((int64_t)b * a.queries + at / a.group) * (a.kv_heads * a.group) + hq) * a.dim + d] =
-        df11_from_float<T>(total == 0.0f ? 0.0f : sum / total);
+    const uint32_t query = at / a.group, hq = head % a.kv_heads * a.group + (at - query * a.group);
+    ((T *)a.out)[(((int64_t)b * a.queries + query) * (a.kv_heads * a.group) + hq) * a.dim + d] =
+        df11_from_float<T>(l == 0.0f ? 0.0f : sum / l);
 }
 
 // How a call is divided, from its sizes alone.
 struct Division {
-    int width, tiles_n, cluster, parts;     // padded head_dim, row tiles of 8, CTAs per cluster, clusters per unit
-    int64_t row_groups, units;
+    int width, tiles_n;         // padded head_dim, row tiles of 8
+    int cluster;                // CTAs per unit; 0: the work is shared out
+    int64_t row_groups, units, ctas, workspace;
 };
+
+constexpr int kSms = 148;
+constexpr double kShareBytes = 16e6;
 
 Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries, int32_t head_dim, int64_t max_slots, int32_t window)
 {
@@ -687,14 +790,43 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
     d.tiles_n = rows > 8 && d.width < 256 ? 2 : 1;
     d.row_groups = (rows + d.tiles_n * 8 - 1) / (d.tiles_n * 8);
     d.units = batch * kv_heads * d.row_groups;
-    const int64_t span = window > 0 && window + queries < max_slots ? window + queries : max_slots;
-    const int64_t tiles = (span + 15) / 16, most = (tiles + 2 * kAttWarps - 1) / (2 * kAttWarps);   // two tiles per warp
-    int64_t want = (900 + d.units - 1) / (d.units > 0 ? d.units : 1);
+    d.workspace = 0;
+    const int64_t span = window > 0 && (int64_t)window + queries < max_slots ? window + queries : max_slots;
+    const int64_t tiles = (span + 15) / 16;
+    const int per_sm = d.width == 256 ? kAttCtas<256, 1> : d.width == 128 ? (d.tiles_n == 1 ? kAttCtas<128, 1> : kAttCtas<128, 2>)
+                                                         : (d.tiles_n == 1 ? kAttCtas<64, 1> : kAttCtas<64, 2>);
+    if ((double)d.units * (double)tiles * d.width * 32 > kShareBytes && (double)d.units * (double)tiles < 2e9) {
+        d.cluster = 0;
+        d.ctas = kSms * per_sm;
+        d.workspace = d.ctas * 2 * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float);
+        return d;
+    }
+    const int64_t most = (tiles + 2 * kAttWarps - 1) / (2 * kAttWarps);                         // two tiles per warp
+    int64_t want = d.units > 0 ? kSms * per_sm / d.units : 1;
     if (want > most) want = most;
     d.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-    d.parts = 1;
-    if (want > 8 && tiles > 8 * 64) d.parts = (int)((want + 7) / 8);
+    d.ctas = d.units * d.cluster;
     return d;
+}
+
+template <typename K> cudaError_t launch_wide(K kernel, unsigned grid, unsigned block, size_t shared, unsigned cluster,
+                                              cudaStream_t stream, const AttentionArgs &a)
+{
+    if (shared > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(block);
+    config.dynamicSmemBytes = shared;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1;
+    return cudaLaunchKernelEx(&config, kernel, a);
 }
 
 template <int D, int NT, int FMT, bool EXACT, typename T>
@@ -703,26 +835,23 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStre
     constexpr int kRows = NT * 8;
     constexpr size_t kJoin = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
     constexpr size_t kRing = (size_t)kAttWarps * kAttStages<D> * (32 * D + 128), kShared = kRing > kJoin ? kRing : kJoin;
-    auto kernel = kv_attention_kernel<D, NT, FMT, EXACT, T>;
-    if (kShared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kShared);
-        if (e != cudaSuccess) return e;
-    }
+    if (d.cluster)
+        return launch_wide(kv_attention_kernel<D, NT, FMT, EXACT, T>, (unsigned)d.ctas, kAttWarps * 32, kShared, (unsigned)d.cluster,
+                           stream, a);
+    const cudaError_t e = launch_wide(kv_attention_shared_kernel<D, NT, FMT, EXACT, T>, (unsigned)d.ctas, kAttWarps * 32, kShared, 1,
+                                      stream, a);
+    if (e != cudaSuccess) return e;
+    // the joining kernel is launched while the first still runs and waits for its end on the device
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(d.units * d.cluster * d.parts));
-    config.blockDim = dim3(kAttWarps * 32);
-    config.dynamicSmemBytes = kShared;
+    config.gridDim = dim3((unsigned)(d.units / d.row_groups * ((int64_t)a.group * a.queries)));
+    config.blockDim = dim3(D);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)d.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
     config.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
-    if (e != cudaSuccess || d.parts == 1) return e;
-    const int64_t heads = d.units / d.row_groups;
-    kv_attention_join_kernel<D, NT, T><<<(unsigned)(heads * ((int64_t)a.group * a.queries)), D, 0, stream>>>(a);
-    return cudaGetLastError();
+    return cudaLaunchKernelEx(&config, kv_attention_join_kernel<D, NT, T>, a, (uint32_t)d.ctas);
 }
 
 template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, cudaStream_t stream)
@@ -842,7 +971,7 @@ extern "C" int64_t df11_kv_attention_workspace_bytes(int64_t batch, int32_t head
         return df11_fail(DF11_ERR_BADARG, "head_dim %d: multiples of 16 up to %d are supported", head_dim, DF11_KV_MAX_HEAD_DIM);
     if ((double)batch * heads * (double)queries > 2e9) return df11_fail(DF11_ERR_BADARG, "too many query rows for one call");
     const Division d = divide(batch, heads, kv_heads, queries, head_dim, max_slots, window);
-    return d.parts > 1 ? d.units * d.parts * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float) : 0;
+    return d.workspace;
 }
 
 extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t,
@@ -870,7 +999,7 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     Df11DeviceScope scope(device);
     if (!scope.ok) return df11_fail(DF11_ERR_CUDA, "cudaSetDevice(%d) failed", device);
     const Division d = divide(batch, heads, kv_heads, queries, head_dim, max_slots, window);
-    if ((double)d.units * d.cluster * d.parts > 2e9) return df11_fail(DF11_ERR_BADARG, "too many query rows for one call");
+    if ((double)d.ctas > 2e9) return df11_fail(DF11_ERR_BADARG, "too many query rows for one call");
     AttentionArgs a = {};
     a.q = q, a.qs = {q_stride_b, q_stride_h, q_stride_t};
     a.q_aligned = !(((uintptr_t)q & 15) || (q_stride_b | q_stride_h | q_stride_t) & 7);
@@ -880,7 +1009,7 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     a.first = (const int64_t *)first, a.first_per = n_first > 1;
     a.out = out, a.workspace = (float *)workspace;
     a.kv_heads = (uint32_t)kv_heads, a.group = (uint32_t)(heads / kv_heads), a.dim = head_dim, a.window = window;
-    a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster, a.parts = (uint32_t)d.parts;
+    a.batch = (uint32_t)batch, a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster;
     a.queries = (uint32_t)queries, a.max_slots = max_slots, a.scale = scale;
     const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, (cudaStream_t)stream)
                                                          : launch_attention<__half>(a, d, format, (cudaStream_t)stream);

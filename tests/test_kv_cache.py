@@ -271,6 +271,41 @@ def test_attention_long(fmt, batch, heads, slots, queries):
 
 
 @gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dim,group,queries,kv_heads,slots,lengths", [
+    (128, 4, 1, 4, 9000, [0, 8999, 1, 0, 0, 17, 300, 9000, 0]),         # one sequence among CTAs, many in one CTA
+    (128, 4, 1, 4, 40000, [39999]),
+    (128, 4, 1, 8, 8000, [0] * 3),                                      # nothing at all
+    (64, 2, 3, 4, 12000, [5, 2500, 0, 2, 4000, 33, 12000]),
+    (256, 5, 4, 2, 9000, [700, 3, 0, 1111]),                            # three row groups
+    (80, 16, 2, 2, 9000, [64, 1000, 0, 2]),
+    (128, 1, 1, 2, 600, [(37 * b) % 600 for b in range(75)]),           # more sequences than a warp has lanes
+    (96, 3, 1, 16, 300, [300 - b % 2 for b in range(70)]),
+])
+@pytest.mark.parametrize("window", [0, 333])
+def test_attention_shared_out(fmt, dim, group, queries, kv_heads, slots, lengths, window):
+    """Caches so large that the tiles of all sequences are shared out evenly; lengths of any kind in them."""
+    batch = len(lengths)
+    shape = (batch, kv_heads, slots, dim)
+    need = _lib.lib.df11_kv_attention_workspace_bytes(batch, kv_heads * group, kv_heads, queries, dim, slots, 0)
+    assert need > 0, "this case is meant to take the shared-out kernel"
+    cache = new_cache(*shape, fmt)
+    g = torch.Generator(device=DEV).manual_seed(40)
+    for c in cache[::2]:
+        for b in range(batch):
+            c[b].copy_((torch.randn(shape[1:], generator=g, device=DEV) * 40).clamp(-127, 127).to(c.dtype))
+    for s in cache[1::2]:
+        s.copy_(torch.rand(s.shape, generator=g, device=DEV) * 0.02)
+    poison(cache, lengths)
+    at = torch.tensor(lengths, device=DEV)
+    q = query(batch, kv_heads * group, queries, dim, torch.bfloat16, 41)
+    got = check_attention(q, cache, at, window=window)
+    assert torch.equal(got, ops.kv_attention(q, *cache, at, window=window))
+    first = torch.tensor([(b * 29) % 50 for b in range(batch)], device=DEV)
+    check_attention(q, cache, at, first=first, window=window)
+
+
+@gpu
 @pytest.mark.parametrize("size", [0.0, 1e-6, 30.0, 1e4])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_attention_flat_and_peaked(size, dtype):
