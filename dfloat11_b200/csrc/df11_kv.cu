@@ -104,9 +104,9 @@ __global__ void __launch_bounds__(128) kv_read_kernel(const uint8_t *k_codes, co
 
 // ---------------------------------------------------------------------------------------------
 // Attention.  For a few query rows per key head the work is reading the cache once: 2 (d + 4) bytes
-// per slot against 4 d multiply-adds per row, so one pass, in which a code goes from memory to one
-// register, is widened to fp16 there (exactly: int8 and e4m3 are subsets of fp16) and meets the
-// matrix unit in that register.  Nothing passes through shared memory:
+// per slot against 4 d multiply-adds per row, so one pass, in which a code is copied to shared memory
+// ahead of time, goes to one register, is widened to fp16 there (exactly: int8 and e4m3 are subsets of
+// fp16) and meets the matrix unit in that register:
 //
 //   scores   S^T[16 slots x 8 rows] += K[16 x 16] Q^T[16 x 8]     (m16n8k16, fp32 sums)
 //   values   O^T[16 dims x 8 rows]  += V^T[16 x 16] P^T[16 x 8]
@@ -150,20 +150,27 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x)
     return y;
 }
 
-// Four codes to two pairs of fp16.  int8: the code plus 128 becomes the bits of a subnormal, so the
-// pair stands for (code + 128) 2^-24, exactly; the products' sums are put right by 128 times the sum of
-// the other operand.  e4m3: the value itself.
-constexpr float kInt8Unit = 0x1p24f;
-template <int FMT> __device__ __forceinline__ void widen(uint32_t codes, uint32_t &lo, uint32_t &hi)
+// Four codes to two pairs of fp16.
+// int8: the code plus 128 becomes the bits of a subnormal, so a number stands for (code + 128) 2^-24,
+// exactly; the products' sums are put right by 128 times the sum of the other operand.
+// e4m3, keys: the conversion instruction, which gives the values themselves at a quarter of the rate of
+// other instructions.  Values: the same with integer instructions -- sign to bit 15, exponent and
+// mantissa to bits 13..7, which stands for the value times 2^-8 --, so that both units share the work.
+constexpr float kInt8Unit = 0x1p24f, kE4m3ValueUnit = 0x1p8f;
+template <int FMT, bool VALUE> __device__ __forceinline__ void widen(uint32_t codes, uint32_t &lo, uint32_t &hi)
 {
     if (FMT == DF11_KV_INT8) {
         const uint32_t u = codes ^ 0x80808080u;
         lo = __byte_perm(u, 0, 0x4140);
         hi = __byte_perm(u, 0, 0x4342);
-    } else {
+    } else if (!VALUE) {
         asm("{ .reg .b16 l, h; mov.b32 {l, h}, %2; cvt.rn.f16x2.e4m3x2 %0, l; cvt.rn.f16x2.e4m3x2 %1, h; }"
             : "=r"(lo), "=r"(hi)
             : "r"(codes));
+    } else {
+        const uint32_t high = (codes & 0x80808080u) | ((codes & 0x7E7E7E7Eu) >> 1), low = (codes << 7) & 0x80808080u;
+        lo = __byte_perm(low, high, 0x5140);
+        hi = __byte_perm(low, high, 0x7362);
     }
 }
 
@@ -182,15 +189,25 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b)
 
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((min(max(e, -126), 127) + 127) << 23); }
 
-// BYTES bytes of one thread: copied to its own place in shared memory ahead of time, read when needed.
+// A warp's tile in shared memory: 16 rows of D bytes in 16-byte chunks.  The chunks of a row are
+// exchanged by its number so that neither way of reading meets a bank twice: keys, 8 lanes taking 4 even
+// (or odd) chunks of two rows; values, 8 lanes taking two chunks of four rows.
+template <int D> __device__ __forceinline__ int chunk_place(int row, int chunk)
+{
+    if (D == 64) {                                          // two rows to a line of 128 bytes
+        const int line = row >> 1;
+        return line * 128 + ((((row & 1) * 4 + chunk) ^ ((line & 3) * 2)) * 16);
+    }
+    return row * D + ((chunk ^ (row & 7)) * 16);
+}
+
+__device__ __forceinline__ void copy_chunk(uint32_t to, const uint8_t *from)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+
 template <int BYTES> struct Bytes {
     uint32_t w[BYTES / 4];
-    static __device__ __forceinline__ void fetch(uint8_t *to, const uint8_t *from)
-    {
-        const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
-        if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
-        else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(BYTES) : "memory");
-    }
     __device__ __forceinline__ void load(const uint8_t *from)
     {
         if (BYTES == 16) {
@@ -342,6 +359,7 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
     float *all_l = all_m + kRows;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, c = lane & 3;
+    auto key_chunk = [&](int j) { return D == 64 ? c : (j >> 1) * 8 + 2 * c + (j & 1); };    // the j-th of this thread
     const uint32_t head = unit / a.row_groups, b = head / a.kv_heads, h = head % a.kv_heads;
     const uint32_t row0 = unit % a.row_groups * kRows, rows = a.group * a.queries, last_row = min(row0 + kRows, rows) - 1;
 
@@ -357,7 +375,7 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
         uint32_t raw[D / 16][2];
 #pragma unroll
         for (int j = 0; j < kKeyChunks; ++j) {
-            const int d0 = (j * 4 + c) * 16;
+            const int d0 = key_chunk(j) * 16;
             if (d0 >= a.dim) {
 #pragma unroll
                 for (int w = 0; w < 4; ++w) raw[j * 4 + w][0] = raw[j * 4 + w][1] = 0;
@@ -444,68 +462,46 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
     for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, f[nt][0] = f[nt][1] = 0x1p126f;
 
     const int dim = EXACT ? D : a.dim;
-    // a thread's places in a tile of 16 slots: key rows r and r + 8, value rows 2c, 2c + 1, 2c + 8, 2c + 9
-    int key_at[kKeyChunks], value_at[kValChunks];
-#pragma unroll
-    for (int j = 0; j < kKeyChunks; ++j) key_at[j] = EXACT ? j * 64 : min((j * 4 + c) * 16, dim - 16);
-#pragma unroll
-    for (int j = 0; j < kValChunks; ++j) value_at[j] = EXACT ? j * 8 * kValBytes : min((j * 8 + r) * kValBytes, dim - kValBytes);
-    const uint8_t *const key_base = a.k_codes + cell0 * dim + (EXACT ? c * 16 : 0);
-    const uint8_t *const value_base = a.v_codes + cell0 * dim + (EXACT ? r * kValBytes : 0);
-    // A warp's tiles come through a ring in shared memory, in which every thread has its own bytes; only
-    // the scales (of keys r and r + 8, of values r and r + 8) are fetched for one another.
-    // Past the last slot the last one is fetched again: its weight is 0 there, and whatever lies in the
-    // cache behind it (a NaN, say) does not reach a product.
+    // A warp's tiles come through a ring in shared memory, each operand of a tile in D / 32 copies of 512
+    // consecutive bytes.  Past the last slot the last one is copied again, and past the last chunk of a
+    // row that one: whatever lies in the cache there (a NaN, say) does not reach a product.
+    constexpr int kRowChunks = D / 16, kRowsPerCopy = 32 / kRowChunks, kCopies = 16 / kRowsPerCopy;
+    const int copy_row = lane / kRowChunks, copy_chunk_at = EXACT ? lane % kRowChunks * 16 : min(lane % kRowChunks * 16, dim - 16);
+    const uint8_t *const key_base = a.k_codes + cell0 * dim + copy_chunk_at, *const value_base = a.v_codes + cell0 * dim + copy_chunk_at;
     uint8_t *const ring = reinterpret_cast<uint8_t *>(shared) + warp * (kStages * kStageBytes);
-    const float *const scale_base = (c < 2 ? a.k_scales : a.v_scales) + cell0;
-    auto fetch = [&](int tile, uint8_t *stage) {
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const float *const scale_base = (c < 2 ? a.k_scales : a.v_scales) + cell0;      // scales of rows r and r + 8, for all lanes of r
+    auto fetch = [&](int tile, uint32_t stage) {
         const int s0 = tile * 16, left = count - 1 - s0;
         const uint8_t *const kp = key_base + (int64_t)s0 * dim, *const vp = value_base + (int64_t)s0 * dim;
-        const int rs = r + 8 * (c & 1);
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(stage + 32 * D + lane * 4)),
-                     "l"(scale_base + s0 + min(rs, left))
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stage + 32 * D + lane * 4),
+                     "l"(scale_base + s0 + min(r + 8 * (c & 1), left))
                      : "memory");
-        if (left >= 15) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < kKeyChunks; ++j)
-                    Bytes<16>::fetch(stage + ((i * kKeyChunks + j) * 32 + lane) * 16, kp + r * dim + 8 * i * dim + key_at[j]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < kValChunks; ++j)
-                    Bytes<kValBytes>::fetch(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes,
-                                            vp + 2 * c * dim + ((i & 1) + 8 * (i >> 1)) * dim + value_at[j]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < kKeyChunks; ++j)
-                    Bytes<16>::fetch(stage + ((i * kKeyChunks + j) * 32 + lane) * 16, kp + min(r + 8 * i, left) * dim + key_at[j]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < kValChunks; ++j)
-                    Bytes<kValBytes>::fetch(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes,
-                                            vp + min(2 * c + (i & 1) + 8 * (i >> 1), left) * dim + value_at[j]);
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = i * kRowsPerCopy + copy_row, from = (left >= 15 ? row : min(row, left)) * dim;
+            const uint32_t to = stage + chunk_place<D>(row, lane % kRowChunks);
+            copy_chunk(to, kp + from);
+            copy_chunk(to + 16 * D, vp + from);
         }
     };
-    int ahead = begin + warp;
+    // which warp takes the first tile differs from CTA to CTA, so that no scheduler gets all the odd ones
+    const int turn_of = (warp + (int)blockIdx.x) & (kAttWarps - 1);
+    int ahead = begin + turn_of;
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
-        if (ahead < end) fetch(ahead, ring + i * kStageBytes);
+        if (ahead < end) fetch(ahead, ring_at + i * kStageBytes);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ahead += kAttWarps;
     }
     int at_stage = 0;
-    for (int tile = begin + warp; tile < end; tile += kAttWarps) {
+    for (int tile = begin + turn_of; tile < end; tile += kAttWarps) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
         __syncwarp();
         const uint8_t *const stage = ring + at_stage * kStageBytes;
         {
             const int to = at_stage == 0 ? kStages - 1 : at_stage - 1;      // read in the step before
-            if (ahead < end) fetch(ahead, ring + to * kStageBytes);
+            if (ahead < end) fetch(ahead, ring_at + to * kStageBytes);
             asm volatile("cp.async.commit_group;" ::: "memory");
             ahead += kAttWarps;
             at_stage = at_stage == kStages - 1 ? 0 : at_stage + 1;
@@ -516,7 +512,7 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int j = 0; j < kKeyChunks; ++j) kx[i][j].load(stage + ((i * kKeyChunks + j) * 32 + lane) * 16);
+            for (int j = 0; j < kKeyChunks; ++j) kx[i][j].load(stage + chunk_place<D>(r + 8 * i, key_chunk(j)));
         float s[NT][4], s2[NT][4] = {};                     // two chains of sums: a product waits for the last of its chain
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][2] = offset[nt][0], s[nt][1] = s[nt][3] = offset[nt][1];
@@ -525,8 +521,8 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 uint32_t a0, a1, a2, a3;
-                widen<FMT>(kx[0][j].w[w], a0, a2);
-                widen<FMT>(kx[1][j].w[w], a1, a3);
+                widen<FMT, false>(kx[0][j].w[w], a0, a2);
+                widen<FMT, false>(kx[1][j].w[w], a1, a3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) mma_16x8x16(w & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][j * 4 + w][0], qf[nt][j * 4 + w][1]);
             }
@@ -534,13 +530,16 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int j = 0; j < kValChunks; ++j) vx[i][j].load(stage + 16 * D + ((i * kValChunks + j) * 32 + lane) * kValBytes);
+            for (int j = 0; j < kValChunks; ++j) {
+                const int row = 2 * c + (i & 1) + 8 * (i >> 1);
+                vx[i][j].load(stage + 16 * D + (kValBytes == 16 ? chunk_place<D>(row, j * 8 + r) : chunk_place<D>(row, r >> 1) + (r & 1) * 8));
+            }
 
         const int s0 = tile * 16;
         const bool whole = s0 >= inner_low && s0 + 15 <= inner_high;    // every row sees every slot
         float p[NT][4], w[NT][4];
         auto weigh = [&]() {                                            // true if a weight has outgrown its bound
-            bool over = false;
+            float most = 0.0f;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -549,9 +548,9 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
                     p[nt][i] = exp2_approx(s[nt][i] - m[nt][col]);
                     w[nt][i] = p[nt][i] * value_scale[i >> 1] * f[nt][col];
                     if (!whole && (slot < col_low[nt][col] || slot > col_high[nt][col])) p[nt][i] = w[nt][i] = 0.0f;
-                    over |= fmaxf(p[nt][i], w[nt][i]) > 16384.0f;
+                    most = fmaxf(most, fmaxf(p[nt][i], w[nt][i]));
                 }
-            return over;
+            return most > 16384.0f;
         };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -611,8 +610,8 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t pick = half ? 0x7362 : 0x5140;       // two dimensions of two slots
                     uint32_t a0, a1, a2, a3;
-                    widen<FMT>(__byte_perm(vx[0][j].w[x], vx[1][j].w[x], pick), a0, a1);
-                    widen<FMT>(__byte_perm(vx[2][j].w[x], vx[3][j].w[x], pick), a2, a3);
+                    widen<FMT, true>(__byte_perm(vx[0][j].w[x], vx[1][j].w[x], pick), a0, a1);
+                    widen<FMT, true>(__byte_perm(vx[2][j].w[x], vx[3][j].w[x], pick), a2, a3);
                     const int k = (j * (kValBytes / 4) + x) * 2 + half;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_16x8x16(o[k][nt], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
@@ -654,7 +653,7 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
             const int row = nt * 8 + 2 * c + col;
             if (row >= live) continue;
             const float turn = (m[nt][col] == -INFINITY ? 1.0f : exp2_approx(m[nt][col] - all_m[row]) / f[nt][col]) *
-                               (FMT == DF11_KV_INT8 ? kInt8Unit : 1.0f);
+                               (FMT == DF11_KV_INT8 ? kInt8Unit : kE4m3ValueUnit);
 #pragma unroll
             for (int k = 0; k < kBlocks; ++k) {
                 // fragment k: this thread's bytes 2k and 2k + 1 of its chunk
@@ -741,31 +740,47 @@ __global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attentio
 }
 
 // Joins the shares of a sequence that was cut, and writes the zeros of one that has no slots: one CTA
-// per query row.
-template <int D, int NT, typename T> __global__ void __launch_bounds__(D) kv_attention_join_kernel(AttentionArgs a, uint32_t ctas)
+// per query row, its threads in kJoinWays ways that take every so-manieth share.
+constexpr int kJoinWays = 4;
+template <int D, int NT, typename T> __global__ void __launch_bounds__(D * kJoinWays) kv_attention_join_kernel(AttentionArgs a, uint32_t ctas)
 {
-    constexpr int kRows = NT * 8;
+    constexpr int kRows = NT * 8, kSlot = kRows * (D + 2);
+    __shared__ float sums[kJoinWays][D], totals[kJoinWays], peaks[kJoinWays];
     const uint32_t rows = a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
     const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, ctas);
     const Sequence s = find_sequence<true>(a, b);
     const uint32_t from = s.before * heads + (head % a.kv_heads * a.row_groups + at / kRows) * s.tiles;
     const uint32_t j0 = from / share, j1 = s.tiles ? (from + s.tiles - 1) / share : j0;
     asm volatile("griddepcontrol.wait;" ::: "memory");                  // the shares are written
-    const int row = (int)(at % kRows), d = threadIdx.x;
-    if (d >= a.dim || (s.tiles && j0 == j1)) return;
-    const float *const first = a.workspace + ((int64_t)j0 * 2 + (j0 * share != from)) * (kRows * (D + 2));
+    if (s.tiles && j0 == j1) return;                                    // whole: written where it was computed
+    const int row = (int)(at % kRows), d = threadIdx.x % D, way = threadIdx.x / D;
     float peak = -INFINITY, sum = 0.0f, l = 0.0f;
     if (s.tiles) {
-        for (uint32_t j = j0; j <= j1; ++j) {
-            const float *part = j == j0 ? first : a.workspace + (int64_t)j * 2 * (kRows * (D + 2));
-            peak = fmaxf(peak, part[kRows * D + row]);
+        // the first share of the sequence may be the second of its CTA, all others are their CTA's first
+        auto part = [&](uint32_t j) { return a.workspace + ((int64_t)j * 2 + (j == j0 && j0 * share != from)) * kSlot; };
+#pragma unroll 4
+        for (uint32_t j = j0 + way; j <= j1; j += kJoinWays) {
+            const float *const x = part(j);
+            const float m = x[kRows * D + row], y = x[row * D + d], z = x[kRows * D + kRows + row];
+            const float now = fmaxf(peak, m), old = peak == -INFINITY ? 0.0f : exp2_approx(peak - now);
+            const float turn = m == -INFINITY ? 1.0f : exp2_approx(m - now);
+            l = l * old + turn * z;
+            sum = sum * old + turn * y;
+            peak = now;
         }
-        for (uint32_t j = j0; j <= j1; ++j) {
-            const float *part = j == j0 ? first : a.workspace + (int64_t)j * 2 * (kRows * (D + 2));
-            const float x = part[kRows * D + row], turn = x == -INFINITY ? 1.0f : exp2_approx(x - peak);
-            l += turn * part[kRows * D + kRows + row];
-            sum += turn * part[row * D + d];
-        }
+    }
+    sums[way][d] = sum;
+    if (d == 0) totals[way] = l, peaks[way] = peak;
+    __syncthreads();
+    if (way || d >= a.dim) return;
+#pragma unroll
+    for (int k = 1; k < kJoinWays; ++k) peak = fmaxf(peak, peaks[k]);
+    sum = l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kJoinWays; ++k) {
+        const float turn = peaks[k] == -INFINITY ? 1.0f : exp2_approx(peaks[k] - peak);
+        l += turn * totals[k];
+        sum += turn * sums[k][d];
     }
     const uint32_t query = at / a.group, hq = head % a.kv_heads * a.group + (at - query * a.group);
     ((T *)a.out)[(((int64_t)b * a.queries + query) * (a.kv_heads * a.group) + hq) * a.dim + d] =
@@ -844,7 +859,7 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStre
     // the joining kernel is launched while the first still runs and waits for its end on the device
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(d.units / d.row_groups * ((int64_t)a.group * a.queries)));
-    config.blockDim = dim3(D);
+    config.blockDim = dim3(D * kJoinWays);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
