@@ -25,7 +25,7 @@
 //
 // A row is divided among a cluster of 1 to 8 CTAs, as many as leave every SM with work.  The row is
 // read two or three times, the first time from memory, then from the L2 cache.  Bound: for few rows the chain of
-// cluster barriers, for many the fp64 units (about 11 operations per token at half a warp per clock).
+// cluster barriers, for many the fp64 units (12 operations per token at half a warp per clock each).
 #include <math.h>
 
 #include "df11_launch.h"
@@ -38,17 +38,16 @@ constexpr int kBins = 4096;
 constexpr int kList = 2048;
 constexpr int kBlocks = kThreads;             // block sums per CTA, at most
 constexpr int kFewTokens = 256;               // top-k up to here goes by the threads' largest
-constexpr uint32_t kLowestKey = 0x00800000u;  // key of the lowest finite float; NaN and -inf lie below
-constexpr uint32_t kInfKey = 0xFF800000u;
+constexpr uint32_t kLowestKey = 0x00800000u;  // key of the lowest finite float
 constexpr uint32_t kAny = 0xFFFFFFFFu;
 
 using u64 = unsigned long long;
 
-// A number that orders like the logit (-0 like 0); 0 for a NaN.
+// A number that orders like the logit (-0 like 0).
 __device__ __forceinline__ uint32_t key_of(float z)
 {
     const uint32_t b = __float_as_uint(z + 0.0f);
-    return z != z ? 0u : (b & 0x80000000u ? ~b : b | 0x80000000u);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
 __device__ __forceinline__ float logit_of(uint32_t key)
@@ -56,15 +55,38 @@ __device__ __forceinline__ float logit_of(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
+// Weights exp((z - c) / T) 2^S, in fp64 to 2^-48 of themselves and rounded to integers.
+// With t = 32 (z - c) / (T ln 2), n the nearest integer and f = t - n:  2^(t/32) = 2^(n/32) 2^(f/32);
+// the first factor is one of 32 numbers times a power of two, the second the Taylor sum of
+// exp(f ln2 / 32) up to the fifth power (|f ln2 / 32| < 0.011, remainder below 3e-15).
+constexpr int kRoots = 32;
 struct Weigher {
-    double peak, inverse, unit;
-    __device__ __forceinline__ double real(uint32_t key) const
+    float best;
+    double peak, slope, unit;
+    int shift;                                // S
+    const double *roots;                      // 2^(j/32), in shared memory
+    __device__ __forceinline__ double real(float z) const
     {
-        const double z = (double)logit_of(key);
-        const double d = z == peak ? 0.0 : z - peak;
-        return d == -INFINITY ? 0.0 : exp(d * inverse);   // beside a +inf; an infinite temperature must not bring it back
+        constexpr double kMagic = 6755399441055744.0;             // 1.5 * 2^52: the sum's low bits are the nearest integer
+        constexpr double a = 0.69314718055994530942 / kRoots;
+        const double t = fmax(((double)z - peak) * slope, -60.0 * kRoots);     // below 2^-60: nothing, also for a NaN
+        const double m = t + kMagic;
+        const int n = __double2loint(m);
+        const double f = t - (m - kMagic);
+        double p = fma(a * a * a * a * a / 120, f, a * a * a * a / 24);
+        p = fma(p, f, a * a * a / 6);
+        p = fma(p, f, a * a / 2);
+        p = fma(p, f, a);
+        const double root = roots[n & (kRoots - 1)];
+        const double scaled = __hiloint2double(__double2hiint(root) + (((n >> 5) + shift) << 20), __double2loint(root));
+        return z == best ? unit : fma(scaled, p * f, scaled);
     }
-    __device__ __forceinline__ u64 operator()(uint32_t key) const { return __double2ull_rn(real(key) * unit); }
+    __device__ __forceinline__ u64 round(double w) const      // w < 2^51
+    {
+        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
+    }
+    __device__ __forceinline__ u64 operator()(float z) const { return round(real(z)); }
+    __device__ __forceinline__ bool dropped(float z, double w, double low) const { return z != best && w < low * unit; }
 };
 
 struct Row {             // settings of a row
@@ -73,12 +95,13 @@ struct Row {             // settings of a row
 };
 
 struct Exchange {        // what the CTAs of a cluster tell one another
-    uint32_t best, least, bound;
+    float best, least, bound;
     u64 mass, above, blocks;
 };
 
 struct Verdict {         // what the first CTA finds on its list
-    uint32_t key, index;                      // kept: keys above, or equal with an index up to this one
+    float logit;                              // kept: logits above, or equal with an index up to this one
+    uint32_t index;
     int fallback;
 };
 
@@ -88,12 +111,13 @@ struct Shared {
     u64 list[kList], weight[kList];
     u64 blocks[kBlocks];
     u64 partial[kWarps];
-    double partial_real[kWarps];
+    double partial_real[kWarps], roots[kRoots];
+    float partial_top[kWarps], partial_bottom[kWarps];
     Exchange mine;
     Verdict verdict;
     uint32_t list_n, found;
-    int bin_k, bin_low, bin_high;             // interval of the top-k border; intervals of the top-p border
-    uint32_t above_k;                         // tokens above bin_k
+    int bin_k, bin_p, bin_low, bin_high;      // interval of the top-k border; of the top-p border, and those around it
+    uint32_t above_k, above_low, upto_high;   // tokens above bin_k; above bin_low; and down to bin_high
     u64 base;
 };
 
@@ -144,9 +168,23 @@ template <typename V> __device__ V block_scan(V x, V *partial, V *total)
     return before + sum - x;
 }
 
-// Sorts list[0 .. n) in descending order (n <= kList); what is behind it, up to a power of two, is lost.
-__device__ void sort_list(u64 *list, int n)
+// Sorts list[0 .. n) of different numbers in descending order (n <= kList); what is behind it, up to a
+// power of two, is lost.
+__device__ __noinline__ void sort_list(u64 *list, int n)
 {
+    if (n <= kThreads / 2) {                  // few: every number's place is how many are larger
+        u64 x = 0;
+        int place = 0;
+        if ((int)threadIdx.x < n) {
+            x = list[threadIdx.x];
+#pragma unroll 8
+            for (int i = 0; i < n; ++i) place += list[i] > x;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < n) list[place] = x;
+        __syncthreads();
+        return;
+    }
     int size = 2;
     while (size < n) size <<= 1;
     for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
@@ -162,19 +200,19 @@ __device__ void sort_list(u64 *list, int n)
         }
 }
 
-__device__ __forceinline__ u64 listed(uint32_t key, uint32_t index) { return (u64)key << 32 | (0xFFFFFFFFu - index); }
-__device__ __forceinline__ uint32_t listed_key(u64 x) { return (uint32_t)(x >> 32); }
+__device__ __forceinline__ u64 listed(float z, uint32_t index) { return (u64)key_of(z) << 32 | (0xFFFFFFFFu - index); }
+__device__ __forceinline__ float listed_logit(u64 x) { return logit_of((uint32_t)(x >> 32)); }
 __device__ __forceinline__ uint32_t listed_index(u64 x) { return 0xFFFFFFFFu - (uint32_t)x; }
 
-// Running sums of weigh(key) over list[0 .. n), in `sums`; the whole sum is returned.
-template <typename K> __device__ u64 scan_list(const u64 *list, int n, u64 *sums, u64 *partial, K key, const Weigher &weigh)
+// Running sums of weigh(logit) over list[0 .. n), in `sums`; the whole sum is returned.
+template <typename K> __device__ u64 scan_list(const u64 *list, int n, u64 *sums, u64 *partial, K logit, const Weigher &weigh)
 {
     constexpr int kEach = kList / kThreads;
     u64 w[kEach], mine = 0, total;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
         const int i = threadIdx.x * kEach + j;
-        w[j] = i < n ? weigh(key(list[i])) : 0;
+        w[j] = i < n ? weigh(logit(list[i])) : 0;
         mine += w[j];
     }
     u64 run = block_scan(mine, partial, &total);
@@ -209,23 +247,23 @@ template <typename T> struct Tokens {
         lead = (int)(reinterpret_cast<uintptr_t>(r) / sizeof(T) % 8);
         groups = (v + lead + 7) / 8;
     }
-    // keys of group g; 0 where there is no token.  Token j of it has the index 8 g - lead + j.
-    __device__ __forceinline__ void keys(uint32_t g, uint32_t (&key)[8]) const
+    // The logits of group g; -inf for a NaN and where there is no token.  Token j of it has the index 8 g - lead + j.
+    __device__ __forceinline__ void logits(uint32_t g, float (&z)[8]) const
     {
         const int64_t first = (int64_t)g * 8 - lead;
         if (first >= 0 && first + 8 <= vocab) {
             uint4 raw[sizeof(T) / 2];
 #pragma unroll
             for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(row + first) + i);
-            const T *z = reinterpret_cast<const T *>(raw);
+            const T *x = reinterpret_cast<const T *>(raw);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) key[j] = key_of(df11_to_float(z[j]));
+            for (int j = 0; j < 8; ++j) z[j] = fmaxf(df11_to_float(x[j]), -INFINITY);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) key[j] = first + j >= 0 && first + j < vocab ? key_of(df11_to_float(row[first + j])) : 0u;
+            for (int j = 0; j < 8; ++j) z[j] = first + j >= 0 && first + j < vocab ? fmaxf(df11_to_float(row[first + j]), -INFINITY) : -INFINITY;
         }
     }
-    __device__ __forceinline__ uint32_t key_at(int64_t i) const { return key_of(df11_to_float(row[i])); }
+    __device__ __forceinline__ float at(int64_t i) const { return fmaxf(df11_to_float(row[i]), -INFINITY); }
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -234,7 +272,7 @@ template <typename T> struct Tokens {
 // The key in which the running measure (from the largest key down) reaches `want`, and the measure
 // above it.
 template <typename T, typename M>
-__device__ void descend(const Tokens<T> &tokens, uint32_t lowest, u64 want, M measure, Shared &s, uint32_t *found, u64 *above)
+__device__ void descend(const Tokens<T> &tokens, float lowest, u64 want, M measure, Shared &s, float *found, u64 *above)
 {
     u64 *digits = s.list;
     uint32_t prefix = 0;
@@ -244,9 +282,10 @@ __device__ void descend(const Tokens<T> &tokens, uint32_t lowest, u64 want, M me
         for (int i = threadIdx.x; i < 256; i += kThreads) digits[i] = 0;
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < tokens.vocab; i += kThreads) {
-            const uint32_t key = tokens.key_at(i);
-            if (key >= lowest && (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)))
-                atomicAdd(&digits[(key >> shift) & 255u], measure(key));
+            const float z = tokens.at(i);
+            const uint32_t key = key_of(z);
+            if (z >= lowest && (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)))
+                atomicAdd(&digits[(key >> shift) & 255u], measure(z));
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -261,28 +300,31 @@ __device__ void descend(const Tokens<T> &tokens, uint32_t lowest, u64 want, M me
         over = s.base;
     }
     __syncthreads();
-    *found = prefix;
+    *found = logit_of(prefix);
     *above = over;
 }
 
-template <typename T> __device__ void sample_slowly(const Tokens<T> &tokens, const Row &row, uint32_t best, uint32_t lowest, const Weigher &weigh,
-                                                    Shared &s, int64_t *out)
+template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T> &tokens, const Row &row, float lowest, const Weigher &weigh, Shared &s, int64_t *out)
 {
     const int tid = threadIdx.x;
     const uint32_t vocab = tokens.vocab;
-    uint32_t kept = lowest;
+    float kept = lowest;
     u64 ties_kept = ~0ull, above, total;
     if (row.k > 0 && row.k < vocab) {
-        descend(tokens, lowest, (u64)row.k, [](uint32_t) { return (u64)1; }, s, &kept, &above);
-        ties_kept = (u64)row.k - min(above, (u64)row.k);
-        if (kept < lowest) kept = lowest, ties_kept = ~0ull;
+        u64 alive = 0;
+        for (uint32_t i = tid; i < vocab; i += kThreads) alive += tokens.at(i) >= lowest;
+        alive = block_sum(alive, s.partial);
+        if ((u64)row.k < alive) {
+            descend(tokens, lowest, (u64)row.k, [](float) { return (u64)1; }, s, &kept, &above);
+            ties_kept = (u64)row.k - above;
+        }
     }
     if (row.p < 1.0) {
         u64 mass = 0, equal = 0;
         for (uint32_t i = tid; i < vocab; i += kThreads) {
-            const uint32_t key = tokens.key_at(i);
-            if (key > kept) mass += weigh(key);
-            equal += key == kept;
+            const float z = tokens.at(i);
+            if (z > kept) mass += weigh(z);
+            equal += z == kept;
         }
         mass = block_sum(mass, s.partial);
         equal = block_sum(equal, s.partial);
@@ -290,11 +332,11 @@ template <typename T> __device__ void sample_slowly(const Tokens<T> &tokens, con
         total = mass + min(equal, ties_kept) * each;
         const u64 want = share_of(row.p, total);
         if (want <= mass) {                       // the border lies above the ties of top-k
-            uint32_t key;
-            const uint32_t before = kept;
-            descend(tokens, lowest, want, [&](uint32_t x) { return x > before ? weigh(x) : (u64)0; }, s, &key, &above);
-            const u64 w = weigh(key);
-            kept = key;
+            float z;
+            const float before = kept;
+            descend(tokens, lowest, want, [&](float x) { return x > before ? weigh(x) : (u64)0; }, s, &z, &above);
+            const u64 w = weigh(z);
+            kept = z;
             ties_kept = (want - above + w - 1) / w;
         } else if (each > 0) {
             ties_kept = min(ties_kept, (want - mass + each - 1) / each);
@@ -303,15 +345,15 @@ template <typename T> __device__ void sample_slowly(const Tokens<T> &tokens, con
     // the draw: every thread has a stretch of the vocabulary, in order
     const uint32_t per = (vocab + kThreads - 1) / kThreads, begin = min(per * tid, vocab), end = min(begin + per, vocab);
     u64 equal = 0;
-    for (uint32_t i = begin; i < end; ++i) equal += tokens.key_at(i) == kept;
+    for (uint32_t i = begin; i < end; ++i) equal += tokens.at(i) == kept;
     u64 ignored;
     const u64 seen = block_scan(equal, s.partial, &ignored);
     auto weight_at = [&](uint32_t i, u64 &ties) -> u64 {
-        const uint32_t key = tokens.key_at(i);
-        if (key < kept || key < lowest) return 0;
-        if (key == kept && ties++ >= ties_kept) return 0;
-        if (row.low > 0.0 && key != best && weigh.real(key) < row.low) return 0;
-        return weigh(key);
+        const float z = tokens.at(i);
+        if (!(z >= kept)) return 0;
+        if (z == kept && ties++ >= ties_kept) return 0;
+        const double w = weigh.real(z);
+        return row.low > 0.0 && weigh.dropped(z, w, row.low) ? 0 : weigh.round(w);
     };
     u64 mine = 0, ties = seen;
     for (uint32_t i = begin; i < end; ++i) mine += weight_at(i, ties);
@@ -330,15 +372,13 @@ template <typename T> __device__ void sample_slowly(const Tokens<T> &tokens, con
 }
 
 // ---------------------------------------------------------------------------------------------
-// The list holds the highest-ranked n tokens of the row, at least those that top-k (or top-p with the mass
-// `total`) keeps: all filters and the draw.  total 0: the mass of what top-k keeps.
-__device__ void draw_from_list(int n, const Row &row, u64 total, uint32_t best, const Weigher &weigh, Shared &s, int64_t *out)
+// The list holds the highest-ranked n tokens of the row, at least those that top-k keeps: all filters and the draw.
+__device__ __noinline__ void draw_from_list(int n, const Row &row, const Weigher &weigh, Shared &s, int64_t *out)
 {
     sort_list(s.list, n);
     if (row.k > 0 && row.k < n) n = (int)row.k;
-    const u64 sum = scan_list(s.list, n, s.weight, s.partial, listed_key, weigh);
     if (row.p < 1.0) {
-        const u64 want = share_of(row.p, total ? total : sum);
+        const u64 want = share_of(row.p, scan_list(s.list, n, s.weight, s.partial, listed_logit, weigh));
         int fit = 0;
         for (int i = threadIdx.x; i < n; i += kThreads) fit += i == 0 || s.weight[i - 1] < want;
         n = (int)block_sum((u64)fit, s.partial);
@@ -346,15 +386,15 @@ __device__ void draw_from_list(int n, const Row &row, u64 total, uint32_t best, 
     if (row.low > 0.0) {
         int fit = 0;
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            const uint32_t key = listed_key(s.list[i]);
-            fit += key == best || weigh.real(key) >= row.low;
+            const float z = listed_logit(s.list[i]);
+            fit += !weigh.dropped(z, weigh.real(z), row.low);
         }
         n = (int)block_sum((u64)fit, s.partial);
     }
     for (int i = threadIdx.x; i < n; i += kThreads) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;   // now by index
     __syncthreads();
     sort_list(s.list, n);
-    const u64 kept = scan_list(s.list, n, s.weight, s.partial, [](u64 x) { return (uint32_t)x; }, weigh);
+    const u64 kept = scan_list(s.list, n, s.weight, s.partial, [](u64 x) { return logit_of((uint32_t)x); }, weigh);
     const u64 want = draw_of(row.u, kept);
     for (int i = threadIdx.x; i < n; i += kThreads)
         if (s.weight[i] > want && (i == 0 || s.weight[i - 1] <= want)) *out = 0xFFFFFFFFu - (uint32_t)(s.list[i] >> 32);
@@ -396,40 +436,53 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     const uint32_t g0 = block0 * block_groups, g1 = min(g0 + blocks * block_groups, tokens.groups);
 
     // the largest and the smallest logit
-    uint32_t top = 0, bottom = kAny;
+    const bool greedy = !(row.t > 0.0), few = !greedy && row.k > 0 && row.k <= kFewTokens;
+    float top = -INFINITY, bottom = INFINITY;
+#pragma unroll 4
     for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-        uint32_t key[8];
-        tokens.keys(g, key);
+        float z[8];
+        tokens.logits(g, z);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            top = max(top, key[j]);
-            if (key[j] >= kLowestKey) bottom = min(bottom, key[j]);
+            top = fmaxf(top, z[j]);
+            bottom = fminf(bottom, z[j] > -INFINITY ? z[j] : INFINITY);
         }
     }
-    if (tid == 0) s.mine.best = 0, s.mine.least = kAny, s.mine.bound = 0, s.list_n = 0;
-    __syncthreads();
+    if (tid < kRoots) s.roots[tid] = exp2((double)tid / kRoots);
+    if (tid == 0) s.mine.bound = -INFINITY, s.list_n = 0, s.found = kAny;
     {
-        const uint32_t t = __reduce_max_sync(0xffffffffu, top), b = __reduce_min_sync(0xffffffffu, bottom);
-        if (lane == 0) atomicMax(&s.mine.best, t), atomicMin(&s.mine.least, b);
+        float x = top, y = bottom;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d)), y = fminf(y, __shfl_xor_sync(0xffffffffu, y, d));
+        if (lane == 0) s.partial_top[warp] = x, s.partial_bottom[warp] = y;
     }
-    const bool greedy = !(row.t > 0.0), few = !greedy && row.k > 0 && row.k <= kFewTokens;
     if (few) {
-        // the largest bound that k of the threads' largest logits reach: at least k tokens reach it, too
+        // a bound that k of the threads' largest logits reach: at least k tokens reach it, too.  Any such
+        // bound will do; the search ends when half as many again reach it
+        const uint32_t key = key_of(top);
         uint32_t low = 0, high = kAny;
         for (int i = 0; i < 32 && low < high; ++i) {
             const uint32_t middle = low + (high - low) / 2 + 1;
-            if (__syncthreads_count(top >= middle) >= row.k) low = middle;
+            const int n = __syncthreads_count(key >= middle);
+            if (n >= row.k) low = middle;
             else high = middle - 1;
+            if (n >= row.k && n <= row.k + row.k / 2) break;
         }
-        if (tid == 0) s.mine.bound = low;
+        if (tid == 0) s.mine.bound = low < kLowestKey ? -INFINITY : logit_of(low);
+    }
+    __syncthreads();
+    if (tid == 0) {
+        float x = -INFINITY, y = INFINITY;
+        for (int w = 0; w < kWarps; ++w) x = fmaxf(x, s.partial_top[w]), y = fminf(y, s.partial_bottom[w]);
+        s.mine.best = x, s.mine.least = y;
     }
     cluster_sync(size);
-    uint32_t best = 0, least = kAny, bound = 0;
+    float best = -INFINITY, least = INFINITY, bound = -INFINITY;
     for (uint32_t r = 0; r < size; ++r) {
         const Exchange *x = size > 1 ? remote(&s.mine, r) : &s.mine;
-        best = max(best, x->best), least = min(least, x->least), bound = max(bound, x->bound);
+        best = fmaxf(best, x->best), least = fminf(least, x->least), bound = fmaxf(bound, x->bound);
     }
-    if (best < kLowestKey) {                                 // nothing to draw from
+    if (best == -INFINITY) {                                 // nothing to draw from
         if (rank == 0 && tid == 0) {
             a.out[at] = 0;
             if (a.status) atomicOr(a.status, DF11_STATUS_EMPTY_ROW);
@@ -440,62 +493,64 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     Shared &head = *(size > 1 ? remote(&s, 0) : &s);
     if (greedy) {
         uint32_t index = kAny;
-        for (uint32_t g = g0 + tid; g < g1 && index == kAny; g += kThreads) {
-            uint32_t key[8];
-            tokens.keys(g, key);
+#pragma unroll 4
+        for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
+            float z[8];
+            tokens.logits(g, z);
 #pragma unroll
-            for (int j = 7; j >= 0; --j)
-                if (key[j] == best) index = g * 8 - tokens.lead + j;
+            for (int j = 0; j < 8; ++j)
+                if (z[j] == best) index = min(index, g * 8 - tokens.lead + j);
         }
-        if (rank == 0 && tid == 0) s.found = kAny;
-        cluster_sync(size);
         index = __reduce_min_sync(0xffffffffu, index);
         if (lane == 0 && index != kAny) atomicMin(&head.found, index);
         cluster_sync(size);
         if (rank == 0 && tid == 0) a.out[at] = s.found;
         return;
     }
-    const uint32_t lowest = best == kInfKey ? best : kLowestKey;        // beside a +inf nothing else is drawn
-    const int bits = 32 - __clz(a.vocab);                               // vocab < 2^bits
-    const Weigher weigh = {(double)logit_of(best), fmin(1.0 / row.t, 1e300), ldexp(1.0, min(63 - bits, 50))};
+    const float lowest = best == INFINITY ? best : -3.402823466e38f;    // beside a +inf nothing else is drawn
+    const int shift = min(31 + __clz(a.vocab), 50);                     // vocab * 2^shift < 2^63
+    const double inverse = fmin(1.0 / row.t, 1e300);
+    const Weigher weigh = {best, (double)best, inverse * (kRoots * 1.4426950408889634074), ldexp(1.0, shift), shift, s.roots};
 
-    auto list_token = [&](uint32_t key, uint32_t index) {
+    auto list_token = [&](float z, uint32_t index) {
         const uint32_t n = atomicAdd(&head.list_n, 1u);
-        if (n < (uint32_t)kList) head.list[n] = listed(key, index);
+        if (n < (uint32_t)kList) head.list[n] = listed(z, index);
     };
     if (few) {
-        bound = max(bound, lowest);
+        bound = fmaxf(bound, lowest);
+#pragma unroll 4
         for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-            uint32_t key[8];
-            tokens.keys(g, key);
+            float z[8];
+            tokens.logits(g, z);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (key[j] >= bound) list_token(key[j], g * 8 - tokens.lead + j);
+                if (z[j] >= bound) list_token(z[j], g * 8 - tokens.lead + j);
         }
         cluster_sync(size);
         if (rank != 0) return;
-        if (s.list_n <= (uint32_t)kList) draw_from_list((int)s.list_n, row, 0, best, weigh, s, a.out + at);
-        else sample_slowly(tokens, row, best, lowest, weigh, s, a.out + at);
+        if (s.list_n <= (uint32_t)kList) draw_from_list((int)s.list_n, row, weigh, s, a.out + at);
+        else sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
         return;
     }
 
-    uint32_t kept_key = lowest, kept_index = kAny;                      // the filters' border so far
+    float kept_logit = lowest;                                          // the filters' border so far
+    uint32_t kept_index = kAny;
+    auto is_kept = [&](float z, uint32_t index) { return z > kept_logit || (z == kept_logit && index <= kept_index); };
     const bool by_rank = row.k > 0, by_mass = row.p < 1.0;
     if (by_rank || by_mass) {
         // tokens per interval
-        const float peak = logit_of(best), range = fminf(peak - logit_of(max(least, lowest)), 31.2f * (float)fmin(row.t, 1e37));
+        const float range = fminf(best - fmaxf(least, lowest), 31.2f * (float)fmin(row.t, 1e37));
         const float scale = range > 0.0f ? fminf((float)kBins / range, 1e30f) : 0.0f;
-        auto bin_of = [&](uint32_t key) {
-            return key == best ? 0 : (int)fminf((peak - logit_of(key)) * scale, (float)(kBins - 1));
-        };
+        auto bin_of = [&](float z) { return z == best ? 0 : (int)fminf((best - z) * scale, (float)(kBins - 1)); };
         for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
         __syncthreads();
+#pragma unroll 2
         for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-            uint32_t key[8];
-            tokens.keys(g, key);
+            float z[8];
+            tokens.logits(g, z);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (key[j] >= lowest) atomicAdd(&s.count[bin_of(key[j])], 1u);
+                if (z[j] >= lowest) atomicAdd(&s.count[bin_of(z[j])], 1u);
         }
         cluster_sync(size);
         if (size > 1) {
@@ -510,51 +565,62 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
 
         // the intervals of the borders; every CTA finds the same ones
         constexpr int kEach = kBins / kThreads;
-        if (tid == 0) s.bin_k = kBins - 1, s.above_k = 0, s.found = kBins - 1;
+        if (tid == 0) {
+            s.bin_k = s.bin_p = s.bin_high = kBins - 1, s.above_k = s.bin_low = s.above_low = 0;
+            s.verdict.fallback = 0;
+        }
         u64 mine = 0, whole;
         for (int j = 0; j < kEach; ++j) mine += count[tid * kEach + j];
-        u64 ahead = block_scan(mine, s.partial, &whole);
+        const u64 ahead = block_scan(mine, s.partial, &whole);
+        if (tid == 0) s.upto_high = (uint32_t)whole;
         const u64 limit = by_rank ? min((u64)row.k, whole) : whole;
-        double mass = 0.0, step = scale > 0.0f ? -1.0 / scale * weigh.inverse : 0.0;
+        const double step = scale > 0.0f ? -1.0 / scale * inverse : 0.0;
+        double mass[kEach], sum = 0.0;
         {
             u64 n = ahead;
+#pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const int bin = tid * kEach + j;
                 const u64 c = count[bin];
                 if (n < limit && n + c >= limit) s.bin_k = bin, s.above_k = (uint32_t)n;
-                if (by_mass && c && n < limit) mass += (double)min(c, limit - n) * exp(step * (bin + 0.5));
+                mass[j] = by_mass && c && n < limit ? (double)min(c, limit - n) * exp(step * (bin + 0.5)) : 0.0;
+                sum += mass[j];
                 n += c;
             }
         }
         if (by_mass) {
-            double all, run = block_scan(mass, s.partial_real, &all);
-            const double want = fmax(row.p, 0.0) * all;
+            // an interval's mass is off by half its width at most, so the border is off by that of all masses
+            double all, run = block_scan(sum, s.partial_real, &all);
+            const double want = fmax(row.p, 0.0) * all, margin = 2.1 * expm1(-0.5 * step) * all;
             u64 n = ahead;
+#pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const int bin = tid * kEach + j;
                 const u64 c = count[bin];
-                if (c && n < limit) {
-                    const double m = (double)min(c, limit - n) * exp(step * (bin + 0.5));
-                    if (run < want && run + m >= want) s.found = (uint32_t)bin;
-                    run += m;
+                const double next = run + mass[j];
+                if (mass[j] > 0.0) {
+                    if (run < want && next >= want) s.bin_p = bin;
+                    if (run < want - margin && next >= want - margin) s.bin_low = bin, s.above_low = (uint32_t)n;
+                    if (run < want + margin && next >= want + margin) s.bin_high = bin, s.upto_high = (uint32_t)(n + c);
                 }
+                run = next;
                 n += c;
             }
         }
-        if (tid == 0) s.verdict.fallback = 0;
         __syncthreads();
         if (by_rank) {
             const int bin = s.bin_k;
             // what top-k keeps, as a whole or the interval of its border
             const bool all = s.above_k + count[bin] <= (uint32_t)kList;
+#pragma unroll 2
             for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-                uint32_t key[8];
-                tokens.keys(g, key);
+                float z[8];
+                tokens.logits(g, z);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (key[j] >= lowest) {
-                        const int b = bin_of(key[j]);
-                        if (b == bin || (all && b < bin)) list_token(key[j], g * 8 - tokens.lead + j);
+                    if (z[j] >= lowest) {
+                        const int b = bin_of(z[j]);
+                        if (b == bin || (all && b < bin)) list_token(z[j], g * 8 - tokens.lead + j);
                     }
             }
             cluster_sync(size);
@@ -562,13 +628,13 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 if (s.list_n > (uint32_t)kList) {
                     if (tid == 0) s.verdict.fallback = 1;
                 } else if (all) {
-                    draw_from_list((int)s.list_n, row, 0, best, weigh, s, a.out + at);
+                    draw_from_list((int)s.list_n, row, weigh, s, a.out + at);
                     if (tid == 0) s.verdict.fallback = 2;
                 } else {
                     sort_list(s.list, (int)s.list_n);
                     if (tid == 0) {
-                        const u64 last = s.list[min(limit, whole) - s.above_k - 1];
-                        s.verdict.key = listed_key(last), s.verdict.index = listed_index(last);
+                        const u64 last = s.list[limit - s.above_k - 1];
+                        s.verdict.logit = listed_logit(last), s.verdict.index = listed_index(last);
                     }
                 }
                 __syncthreads();
@@ -578,54 +644,52 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             const Verdict v = head.verdict;
             if (v.fallback) {
                 cluster_sync(size);
-                if (v.fallback == 1 && rank == 0) sample_slowly(tokens, row, best, lowest, weigh, s, a.out + at);
+                if (v.fallback == 1 && rank == 0) sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
                 return;
             }
-            kept_key = v.key, kept_index = v.index;
+            kept_logit = v.logit, kept_index = v.index;
         }
         if (by_mass) {
-            // as many intervals around the likely border as the list has room for, up to four on either side
-            if (tid == 0) {
-                int low = (int)s.found, high = low;
+            // all intervals in which the border can lie, or as many around the likely one as the list takes
+            if (tid == 0 && s.upto_high - s.above_low > (uint32_t)kList) {
+                int low = s.bin_p, high = low;
                 uint32_t n = count[low];
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) {
                     if (low > 0 && n + count[low - 1] <= (uint32_t)kList) n += count[--low];
                     if (high < kBins - 1 && n + count[high + 1] <= (uint32_t)kList) n += count[++high];
                 }
                 s.bin_low = low, s.bin_high = high;
             }
             __syncthreads();
-        }
-        // one pass: mass of what top-k keeps, mass above the intervals, sums of blocks of the latter
-        if (by_mass) {
+            // one pass: mass of what top-k keeps, mass above the intervals, sums of blocks of the latter
             const int low = s.bin_low, high = s.bin_high;
             u64 mass_all = 0, mass_above = 0;
             for (uint32_t block = warp; block < blocks; block += kWarps) {
-                u64 sum = 0;
+                u64 part = 0;
                 for (int x = 0; x < 1 << wide; ++x) {
                     const uint32_t g = g0 + block * block_groups + x * 32 + lane;
                     if (g >= g1) continue;
-                    uint32_t key[8];
-                    tokens.keys(g, key);
+                    float z[8];
+                    tokens.logits(g, z);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t index = g * 8 - tokens.lead + j;
-                        if (key[j] < kept_key || (key[j] == kept_key && index > kept_index)) continue;
-                        const int b = bin_of(key[j]);
-                        const double real = weigh.real(key[j]);
-                        const u64 w = __double2ull_rn(real * weigh.unit);
+                        if (!is_kept(z[j], index)) continue;
+                        const int b = bin_of(z[j]);
+                        const double real = weigh.real(z[j]);
+                        const u64 w = weigh.round(real);
                         mass_all += w;
                         if (b < low) {
                             mass_above += w;
-                            if (!(row.low > 0.0 && key[j] != best && real < row.low)) sum += w;
+                            if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) part += w;
                         } else if (b <= high) {
-                            list_token(key[j], index);
+                            list_token(z[j], index);
                         }
                     }
                 }
 #pragma unroll
-                for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-                if (lane == 0) s.blocks[block] = sum;
+                for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+                if (lane == 0) s.blocks[block] = part;
             }
             mass_all = block_sum(mass_all, s.partial);
             mass_above = block_sum(mass_above, s.partial);
@@ -640,16 +704,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 const u64 want = share_of(row.p, mass_all);
                 const int n = (int)min(s.list_n, (uint32_t)kList);
                 sort_list(s.list, n);
-                const u64 sum = scan_list(s.list, n, s.weight, s.partial, listed_key, weigh);
-                if (s.list_n > (uint32_t)kList || mass_above >= want || mass_above + sum < want) {
+                const u64 on_list = scan_list(s.list, n, s.weight, s.partial, listed_logit, weigh);
+                if (s.list_n > (uint32_t)kList || mass_above >= want || mass_above + on_list < want) {
                     if (tid == 0) s.verdict.fallback = 1;
                 } else {
                     for (int i = tid; i < n; i += kThreads) {
                         const u64 before = mass_above + (i ? s.weight[i - 1] : 0), after = mass_above + s.weight[i];
                         if (before >= want) continue;
-                        const uint32_t key = listed_key(s.list[i]), index = listed_index(s.list[i]);
-                        if (after >= want) s.verdict.key = key, s.verdict.index = index;
-                        if (row.low > 0.0 && key != best && weigh.real(key) < row.low) continue;
+                        const float z = listed_logit(s.list[i]);
+                        const uint32_t index = listed_index(s.list[i]);
+                        if (after >= want) s.verdict.logit = z, s.verdict.index = index;
+                        if (row.low > 0.0 && weigh.dropped(z, weigh.real(z), row.low)) continue;
                         const uint32_t block = (index + tokens.lead) / 8 / block_groups, owner = block / my_blocks;
                         atomicAdd(&(size > 1 ? remote(&s, owner) : &s)->blocks[block - owner * my_blocks], after - before);
                     }
@@ -659,31 +724,30 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             const Verdict v = head.verdict;
             if (v.fallback) {
                 cluster_sync(size);
-                if (rank == 0) sample_slowly(tokens, row, best, lowest, weigh, s, a.out + at);
+                if (rank == 0) sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
                 return;
             }
-            kept_key = v.key, kept_index = v.index;
+            kept_logit = v.logit, kept_index = v.index;
         }
     }
     if (!by_mass) {
         for (uint32_t block = warp; block < blocks; block += kWarps) {
-            u64 sum = 0;
+            u64 part = 0;
             for (int x = 0; x < 1 << wide; ++x) {
                 const uint32_t g = g0 + block * block_groups + x * 32 + lane;
                 if (g >= g1) continue;
-                uint32_t key[8];
-                tokens.keys(g, key);
+                float z[8];
+                tokens.logits(g, z);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (key[j] < kept_key || (key[j] == kept_key && g * 8 - tokens.lead + j > kept_index)) continue;
-                    const double real = weigh.real(key[j]);
-                    if (row.low > 0.0 && key[j] != best && real < row.low) continue;
-                    sum += __double2ull_rn(real * weigh.unit);
+                    if (!is_kept(z[j], g * 8 - tokens.lead + j)) continue;
+                    const double real = weigh.real(z[j]);
+                    if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) part += weigh.round(real);
                 }
             }
 #pragma unroll
-            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            if (lane == 0) s.blocks[block] = sum;
+            for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+            if (lane == 0) s.blocks[block] = part;
         }
     }
     // the draw: the CTA, the block, the token
@@ -707,16 +771,16 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             run = s.base;
             for (int x = 0; x < 1 << wide; ++x) {
                 const uint32_t g = g0 + s.found * block_groups + x * 32 + lane;
-                uint32_t key[8] = {};
-                if (g < g1) tokens.keys(g, key);
+                float z[8];
+                if (g < g1) tokens.logits(g, z);
                 u64 w[8];
                 sum = 0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     w[j] = 0;
-                    if (key[j] >= kept_key && !(key[j] == kept_key && g * 8 - tokens.lead + j > kept_index)) {
-                        const double real = weigh.real(key[j]);
-                        if (!(row.low > 0.0 && key[j] != best && real < row.low)) w[j] = __double2ull_rn(real * weigh.unit);
+                    if (g < g1 && is_kept(z[j], g * 8 - tokens.lead + j)) {
+                        const double real = weigh.real(z[j]);
+                        if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) w[j] = weigh.round(real);
                     }
                     sum += w[j];
                 }
