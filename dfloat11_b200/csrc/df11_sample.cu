@@ -60,16 +60,29 @@ __device__ __forceinline__ float logit_of(uint32_t key)
 // the first factor is one of 32 numbers times a power of two, the second the Taylor sum of
 // exp(f ln2 / 32) up to the fifth power (|f ln2 / 32| < 0.011, remainder below 3e-15).
 constexpr int kRoots = 32;
+constexpr double kOne52 = 4503599627370496.0;  // 2^52: added to a number below it, the sum's low bits are the nearest integer
 struct Weigher {
-    float best;
+    float best, cap, cut;                     // cut: below, a weight is less than 2^-60 and taken as 0
     double peak, slope, unit;
     int shift;                                // S
     const double *roots;                      // 2^(j/32), in shared memory
+
+    __device__ __forceinline__ Weigher(float b, double t, int s, const double *r) : best(b), shift(s), roots(r)
+    {
+        const double inverse = fmin(1.0 / t, 1e300);
+        cap = b == INFINITY ? 0.0f : b;       // beside a +inf only its like have a weight
+        cut = b == INFINITY ? b : fmaxf((float)(b - 60.0 * 0.69314718055994530942 * t), -3.402823466e38f);
+        peak = (double)cap;
+        slope = inverse * (kRoots * 1.4426950408889634074);
+        unit = ldexp(1.0, s);
+    }
+    // 0 for a NaN and for -inf; exactly 2^S for the largest
     __device__ __forceinline__ double real(float z) const
     {
-        constexpr double kMagic = 6755399441055744.0;             // 1.5 * 2^52: the sum's low bits are the nearest integer
+        constexpr double kMagic = 1.5 * kOne52;
         constexpr double a = 0.69314718055994530942 / kRoots;
-        const double t = fmax(((double)z - peak) * slope, -60.0 * kRoots);     // below 2^-60: nothing, also for a NaN
+        const bool some = z >= cut;
+        const double t = ((double)fminf(some ? z : best, cap) - peak) * slope;
         const double m = t + kMagic;
         const int n = __double2loint(m);
         const double f = t - (m - kMagic);
@@ -79,14 +92,12 @@ struct Weigher {
         p = fma(p, f, a);
         const double root = roots[n & (kRoots - 1)];
         const double scaled = __hiloint2double(__double2hiint(root) + (((n >> 5) + shift) << 20), __double2loint(root));
-        return z == best ? unit : fma(scaled, p * f, scaled);
+        return some ? fma(scaled, p * f, scaled) : 0.0;
     }
-    __device__ __forceinline__ u64 round(double w) const      // w < 2^51
-    {
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xFFFFFFFFFFFFFull;
-    }
-    __device__ __forceinline__ u64 operator()(float z) const { return round(real(z)); }
-    __device__ __forceinline__ bool dropped(float z, double w, double low) const { return z != best && w < low * unit; }
+    // The nearest integer to w < 2^51, plus kBias; sums of such numbers are put right by as many kBias.
+    static constexpr u64 kBias = 0x4330000000000000ull;
+    __device__ __forceinline__ static u64 biased(double w) { return (u64)__double_as_longlong(w + kOne52); }
+    __device__ __forceinline__ u64 operator()(float z) const { return biased(real(z)) - kBias; }
 };
 
 struct Row {             // settings of a row
@@ -343,6 +354,7 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
         }
     }
     // the draw: every thread has a stretch of the vocabulary, in order
+    const double floor = row.low * weigh.unit;
     const uint32_t per = (vocab + kThreads - 1) / kThreads, begin = min(per * tid, vocab), end = min(begin + per, vocab);
     u64 equal = 0;
     for (uint32_t i = begin; i < end; ++i) equal += tokens.at(i) == kept;
@@ -353,7 +365,7 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
         if (!(z >= kept)) return 0;
         if (z == kept && ties++ >= ties_kept) return 0;
         const double w = weigh.real(z);
-        return row.low > 0.0 && weigh.dropped(z, w, row.low) ? 0 : weigh.round(w);
+        return w < floor ? 0 : weigh.biased(w) - weigh.kBias;
     };
     u64 mine = 0, ties = seen;
     for (uint32_t i = begin; i < end; ++i) mine += weight_at(i, ties);
@@ -383,11 +395,11 @@ __device__ __noinline__ void draw_from_list(int n, const Row &row, const Weigher
         for (int i = threadIdx.x; i < n; i += kThreads) fit += i == 0 || s.weight[i - 1] < want;
         n = (int)block_sum((u64)fit, s.partial);
     }
-    if (row.low > 0.0) {
+    if (row.low > 0.0) {                      // min-p
         int fit = 0;
         for (int i = threadIdx.x; i < n; i += kThreads) {
             const float z = listed_logit(s.list[i]);
-            fit += !weigh.dropped(z, weigh.real(z), row.low);
+            fit += weigh.real(z) >= row.low * weigh.unit;
         }
         n = (int)block_sum((u64)fit, s.partial);
     }
@@ -422,7 +434,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     row.t = a.temperature ? (double)a.temperature[at] : a.temperature_value;
     row.k = a.top_k ? a.top_k[at] : a.top_k_value;
     row.p = a.top_p ? (double)a.top_p[at] : a.top_p_value;
-    row.low = fmin(a.min_p ? (double)a.min_p[at] : a.min_p_value, 1.0);
+    row.low = a.min_p ? (double)a.min_p[at] : a.min_p_value;
+    row.low = row.low > 0.0 ? fmin(row.low, 1.0) : 0.0;
     row.u = (double)a.uniform[at];
     if (row.k >= a.vocab) row.k = 0;
     const Tokens<T> tokens((const T *)a.logits + (int64_t)at * a.stride, a.vocab);
@@ -509,8 +522,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     }
     const float lowest = best == INFINITY ? best : -3.402823466e38f;    // beside a +inf nothing else is drawn
     const int shift = min(31 + __clz(a.vocab), 50);                     // vocab * 2^shift < 2^63
-    const double inverse = fmin(1.0 / row.t, 1e300);
-    const Weigher weigh = {best, (double)best, inverse * (kRoots * 1.4426950408889634074), ldexp(1.0, shift), shift, s.roots};
+    const Weigher weigh(best, row.t, shift, s.roots);
+    const double floor = row.low * weigh.unit;                          // weights below it are min-p's
 
     auto list_token = [&](float z, uint32_t index) {
         const uint32_t n = atomicAdd(&head.list_n, 1u);
@@ -574,7 +587,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
         const u64 ahead = block_scan(mine, s.partial, &whole);
         if (tid == 0) s.upto_high = (uint32_t)whole;
         const u64 limit = by_rank ? min((u64)row.k, whole) : whole;
-        const double step = scale > 0.0f ? -1.0 / scale * inverse : 0.0;
+        const double step = scale > 0.0f ? -fmin(1.0 / row.t, 1e300) / scale : 0.0;
         double mass[kEach], sum = 0.0;
         {
             u64 n = ahead;
@@ -662,29 +675,33 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             }
             __syncthreads();
             // one pass: mass of what top-k keeps, mass above the intervals, sums of blocks of the latter
-            const int low = s.bin_low, high = s.bin_high;
+            const float low = (float)s.bin_low, high = s.bin_high == kBins - 1 ? INFINITY : (float)(s.bin_high + 1);
             u64 mass_all = 0, mass_above = 0;
             for (uint32_t block = warp; block < blocks; block += kWarps) {
                 u64 part = 0;
                 for (int x = 0; x < 1 << wide; ++x) {
-                    const uint32_t g = g0 + block * block_groups + x * 32 + lane;
+                    const uint32_t g = g0 + block * block_groups + x * 32 + lane, index = g * 8 - tokens.lead;
                     if (g >= g1) continue;
                     float z[8];
                     tokens.logits(g, z);
+                    uint32_t on_list = 0;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const uint32_t index = g * 8 - tokens.lead + j;
-                        if (!is_kept(z[j], index)) continue;
-                        const int b = bin_of(z[j]);
-                        const double real = weigh.real(z[j]);
-                        const u64 w = weigh.round(real);
-                        mass_all += w;
-                        if (b < low) {
-                            mass_above += w;
-                            if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) part += w;
-                        } else if (b <= high) {
-                            list_token(z[j], index);
-                        }
+                        const bool kept = is_kept(z[j], index + j);
+                        const float interval = z[j] == best ? 0.0f : (best - z[j]) * scale;
+                        const bool over = kept && interval < low;
+                        const double w = weigh.real(z[j]);
+                        const u64 all = weigh.biased(kept ? w : 0.0);
+                        mass_all += all;
+                        mass_above += over ? all : weigh.kBias;
+                        part += over && w >= floor ? all : weigh.kBias;
+                        if (kept && !over && interval < high) on_list |= 1u << j;
+                    }
+                    mass_all -= 8 * weigh.kBias, mass_above -= 8 * weigh.kBias, part -= 8 * weigh.kBias;
+                    if (on_list) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (on_list >> j & 1) list_token(z[j], index + j);
                     }
                 }
 #pragma unroll
@@ -714,7 +731,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                         const float z = listed_logit(s.list[i]);
                         const uint32_t index = listed_index(s.list[i]);
                         if (after >= want) s.verdict.logit = z, s.verdict.index = index;
-                        if (row.low > 0.0 && weigh.dropped(z, weigh.real(z), row.low)) continue;
+                        if (weigh.real(z) < floor) continue;
                         const uint32_t block = (index + tokens.lead) / 8 / block_groups, owner = block / my_blocks;
                         atomicAdd(&(size > 1 ? remote(&s, owner) : &s)->blocks[block - owner * my_blocks], after - before);
                     }
@@ -740,10 +757,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 tokens.logits(g, z);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    if (!is_kept(z[j], g * 8 - tokens.lead + j)) continue;
-                    const double real = weigh.real(z[j]);
-                    if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) part += weigh.round(real);
+                    const double w = weigh.real(z[j]);
+                    part += weigh.biased(is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor ? w : 0.0);
                 }
+                part -= 8 * weigh.kBias;
             }
 #pragma unroll
             for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
@@ -780,7 +797,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     w[j] = 0;
                     if (g < g1 && is_kept(z[j], g * 8 - tokens.lead + j)) {
                         const double real = weigh.real(z[j]);
-                        if (!(row.low > 0.0 && weigh.dropped(z[j], real, row.low))) w[j] = weigh.round(real);
+                        if (real >= floor) w[j] = weigh.biased(real) - weigh.kBias;
                     }
                     sum += w[j];
                 }
