@@ -15,22 +15,6 @@
 
 namespace {
 
-__device__ __forceinline__ float top_of(int format) { return format == DF11_KV_INT8 ? 127.0f : 448.0f; }
-
-__device__ __forceinline__ float code_value(uint8_t code, int format)
-{
-    if (format == DF11_KV_INT8) return (float)(int8_t)code;
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(code, __NV_E4M3);
-    return __half2float(__half(h));
-}
-
-__device__ __forceinline__ float warp_max(float x)
-{
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-    return x;
-}
-
 // A length or a first slot as the user's program may have it; what is beyond any cache must not
 // overflow in what is computed from it.
 __device__ __forceinline__ int64_t clamped_length(int64_t n) { return n < 0 ? 0 : n > (1ll << 40) ? 1ll << 40 : n; }
@@ -39,67 +23,187 @@ struct Strides {
     int64_t b, h, t;
 };
 
-// One warp per row of k or v.
-template <typename T>
-__global__ void __launch_bounds__(128) kv_append_kernel(const T *k, const T *v, Strides ks, Strides vs, uint8_t *k_codes,
-                                                        float *k_scales, uint8_t *v_codes, float *v_scales,
-                                                        const int64_t *positions, int per_sequence, int64_t rows,
-                                                        int heads, int64_t tokens, int dim, int64_t max_slots, int format,
-                                                        int *status)
+// Writing and reading move bytes and compute little: 3 bytes per number either way.  A group of LANES
+// threads (a power of two) holds a row in registers, 16 numbers per thread, so that a row's maximum is a few
+// shuffles and its codes leave as one 16-byte store per thread.
+// 16 numbers from an address that may have any alignment of the type.
+template <typename T> __device__ __forceinline__ void load16(const T *p, bool aligned, uint4 (&raw)[2])
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= 2 * rows) return;
-    const bool value = row >= rows;
-    const int64_t r = value ? row - rows : row;
-    const int64_t t = r % tokens, h = r / tokens % heads, b = r / tokens / heads;
-    const Strides s = value ? vs : ks;
-    const T *x = (value ? v : k) + b * s.b + h * s.h + t * s.t;
-    const int64_t position = positions[per_sequence ? b : 0];
-    if (position < -t || position >= max_slots - t) {
-        if (lane == 0 && status) atomicOr(status, DF11_STATUS_BAD_POSITIONS);
-        return;
+    if (aligned) {
+        raw[0] = __ldg(reinterpret_cast<const uint4 *>(p)), raw[1] = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+    } else {
+        const uint16_t *y = reinterpret_cast<const uint16_t *>(p);
+        uint32_t *w = reinterpret_cast<uint32_t *>(raw);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = (uint32_t)y[2 * i] | (uint32_t)y[2 * i + 1] << 16;
     }
-    const int64_t slot = position + t;
-    float a = 0.0f;
-    bool finite = true;
-    for (int i = lane; i < dim; i += 32) {
-        const float m = fabsf(df11_to_float(x[i]));
-        finite &= m <= 3.402823466e38f;
-        a = fmaxf(a, m);
-    }
-    a = warp_max(a);
-    finite = __all_sync(0xffffffffu, finite);
-    const float top = top_of(format);
-    const int64_t cell = (b * heads + h) * max_slots + slot;
-    uint8_t *codes = (value ? v_codes : k_codes) + cell * dim;
-    // a power of two that keeps x * top away from overflow and x away from the subnormals
-    const float shift = a > 1e30f ? 0x1p-40f : a < 1e-30f ? 0x1p40f : 1.0f;
-    for (int i = lane; i < dim; i += 32) {
-        float q = 0.0f;
-        if (finite && a > 0.0f) q = __fdiv_rn(df11_to_float(x[i]) * shift * top, a * shift);
-        codes[i] = format == DF11_KV_INT8 ? (uint8_t)(int8_t)__float2int_rn(q)
-                                          : (uint8_t)__nv_cvt_float_to_fp8(q, __NV_SATFINITE, __NV_E4M3);
-    }
-    if (lane == 0) (value ? v_scales : k_scales)[cell] = finite ? __fdiv_rn(a, top) : __int_as_float(0x7fc00000);
 }
 
-// One warp per row of the result.
-template <typename T>
-__global__ void __launch_bounds__(128) kv_read_kernel(const uint8_t *k_codes, const float *k_scales, const uint8_t *v_codes,
-                                                      const float *v_scales, T *k_out, T *v_out, int64_t rows,
-                                                      int64_t max_slots, int dim, int64_t first, int64_t n, int format)
+struct AppendArgs {
+    const void *k, *v;
+    Strides ks, vs;
+    uint8_t *k_codes, *v_codes;
+    float *k_scales, *v_scales;
+    const int64_t *positions;
+    int *status;
+    int64_t max_slots;
+    uint32_t batch, heads, tokens;
+    int per_sequence, dim, aligned;
+};
+
+template <typename T> constexpr uint32_t kInfBits = 0;
+template <> constexpr uint32_t kInfBits<__nv_bfloat16> = 0x7F80;
+template <> constexpr uint32_t kInfBits<__half> = 0x7C00;
+
+// The codes of x * up / over.  A product with the reciprocal is off by 2^-21 of itself at most; only where
+// that could decide (one number in some thousands), or where `extreme` says that the factor does not fit a
+// float, is the quotient itself computed.
+template <int FMT> __device__ __forceinline__ uint32_t codes_of(const float (&x)[4], float up, float over, float factor, bool extreme)
 {
-    const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (row >= 2 * rows) return;
-    const bool value = row >= rows;
-    const int64_t r = value ? row - rows : row;
-    const int64_t cell = r / n * max_slots + first + r % n;
-    const uint8_t *codes = (value ? v_codes : k_codes) + cell * dim;
-    const float scale = (value ? v_scales : k_scales)[cell];
-    T *out = (value ? v_out : k_out) + r * dim;
-    for (int i = lane; i < dim; i += 32) out[i] = df11_from_float<T>(code_value(codes[i], format) * scale);
+    constexpr float kMagic = 12582912.0f;       // 1.5 * 2^23: the sum's low bits are the nearest integer
+    uint32_t y;
+    bool close;
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = x[i] * factor;
+    if (FMT == DF11_KV_INT8) {
+        uint32_t n[4];
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float m = q[i] + kMagic;
+            n[i] = __float_as_uint(m);
+            far = fmaxf(far, fabsf(q[i] - (m - kMagic)));
+        }
+        y = __byte_perm(__byte_perm(n[0], n[1], 0x0040), __byte_perm(n[2], n[3], 0x0040), 0x5410);
+        close = far > 0.4999f;                  // 127 * 2^-21 < 0.0001
+    } else {
+        auto pack = [&](float scale) {
+            return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[0] * scale, q[1] * scale), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[2] * scale, q[3] * scale), __NV_SATFINITE, __NV_E4M3) << 16;
+        };
+        y = pack(1.0f - 0x1p-20f);
+        close = y != pack(1.0f + 0x1p-20f);
+    }
+    if (close || extreme) {
+        y = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float exact = __fdiv_rn(x[i] * up, over);
+            y |= (FMT == DF11_KV_INT8 ? (uint32_t)(__float2int_rn(exact) & 255)
+                                      : (uint32_t)__nv_cvt_float_to_fp8(exact, __NV_SATFINITE, __NV_E4M3)) << (8 * i);
+        }
+    }
+    return y;
+}
+
+// One block: rows of one sequence (blockIdx.y, and every gridDim.y-th after it); the value rows follow the
+// key rows.
+template <int LANES, int FMT, typename T> __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a)
+{
+    constexpr int kRows = 256 / LANES;
+    const uint32_t per = a.heads * a.tokens, r = blockIdx.x * kRows + threadIdx.x / LANES;
+    const int part = threadIdx.x % LANES * 16;
+    const bool value = r >= per, some = r < 2 * per;
+    const uint32_t within = some ? (value ? r - per : r) : 0, t = within / a.heads, h = within - t * a.heads;
+    const bool mine = some && part < a.dim;
+    for (uint32_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+        const int64_t position = a.positions[a.per_sequence ? b : 0];
+        const bool there = position >= -(int64_t)t && position < a.max_slots - (int64_t)t;
+        uint4 raw[2] = {};
+        if (mine && there) {
+            const Strides s = value ? a.vs : a.ks;
+            load16((const T *)(value ? a.v : a.k) + b * s.b + h * s.h + t * s.t + part, a.aligned, raw);
+        }
+        // magnitudes order like their bits, a NaN above an infinity
+        uint32_t bits = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) bits = __vmaxu2(bits, reinterpret_cast<const uint32_t *>(raw)[w] & 0x7FFF7FFFu);
+#pragma unroll
+        for (int d = LANES / 2; d; d >>= 1) bits = __vmaxu2(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+        bits = max(bits & 0xFFFFu, bits >> 16);
+        if (!mine) continue;
+        if (!there) {
+            if (part == 0 && a.status) atomicOr(a.status, DF11_STATUS_BAD_POSITIONS);
+            continue;
+        }
+        const bool finite = bits < kInfBits<T>, zero = bits == 0 || !finite;
+        const uint16_t top_bits = (uint16_t)bits;
+        const float most = FMT == DF11_KV_INT8 ? 127.0f : 448.0f, top = df11_to_float(*reinterpret_cast<const T *>(&top_bits));
+        // a power of two that keeps x * most away from overflow and x away from the subnormals
+        const float shift = top > 1e30f ? 0x1p-40f : top < 1e-30f ? 0x1p40f : 1.0f;
+        const float over = zero ? 1.0f : top * shift, up = shift * most, factor = up * __frcp_rn(over);
+        uint32_t codes[4];
+        const T *const x = reinterpret_cast<const T *>(raw);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float four[4] = {df11_to_float(x[4 * w]), df11_to_float(x[4 * w + 1]), df11_to_float(x[4 * w + 2]), df11_to_float(x[4 * w + 3])};
+            codes[w] = zero ? 0 : codes_of<FMT>(four, up, over, factor, shift != 1.0f);
+        }
+        const int64_t cell = ((int64_t)b * a.heads + h) * a.max_slots + position + t;
+        *reinterpret_cast<uint4 *>((value ? a.v_codes : a.k_codes) + cell * a.dim + part) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+        if (part == 0) (value ? a.v_scales : a.k_scales)[cell] = finite ? __fdiv_rn(top, most) : __int_as_float(0x7fc00000);
+    }
+}
+
+struct ReadArgs {
+    const uint8_t *k_codes, *v_codes;
+    const float *k_scales, *v_scales;
+    void *k_out, *v_out;
+    int64_t max_slots, first;
+    uint32_t units, n, chunks;          // heads of all sequences, slots read, 8-byte chunks per row
+};
+
+// A thread takes 8 codes at a time, so that a warp's stores cover consecutive bytes, kEach times for loads
+// in flight; blockIdx.y is the head of a sequence, blockIdx.z keys or values.
+template <int FMT, typename T> __global__ void __launch_bounds__(256) kv_read_kernel(ReadArgs a)
+{
+    constexpr int kEach = 4;
+    const uint64_t all = (uint64_t)a.n * a.chunks, i0 = (uint64_t)blockIdx.x * (256 * kEach) + threadIdx.x;
+    for (int64_t unit = blockIdx.y; unit < a.units; unit += gridDim.y) {
+        const uint8_t *const codes = (blockIdx.z ? a.v_codes : a.k_codes) + (unit * a.max_slots + a.first) * a.chunks * 8;
+        const float *const scales = (blockIdx.z ? a.v_scales : a.k_scales) + unit * a.max_slots + a.first;
+        T *const out = (T *)(blockIdx.z ? a.v_out : a.k_out) + unit * a.n * a.chunks * 8;
+        uint2 raw[kEach];
+        float scale[kEach];
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const uint64_t i = i0 + e * 256;
+            if (i >= all) continue;
+            raw[e] = __ldg(reinterpret_cast<const uint2 *>(codes) + i);
+            scale[e] = __ldg(scales + (a.chunks == 16 ? i >> 4 : i / a.chunks));
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const uint64_t i = i0 + e * 256;
+            if (i >= all) continue;
+            const uint32_t words[2] = {raw[e].x, raw[e].y};
+            __align__(16) T y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t code = words[k / 4] >> (8 * (k % 4));
+                float x;
+                if (FMT == DF11_KV_INT8) x = (float)(int8_t)code;
+                else x = __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)code, __NV_E4M3)));
+                y[k] = df11_from_float<T>(x * scale[e]);
+            }
+            reinterpret_cast<uint4 *>(out)[i] = *reinterpret_cast<const uint4 *>(y);
+        }
+    }
+}
+
+template <int LANES, typename T> void launch_append(const AppendArgs &a, int format, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)(((uint64_t)2 * a.heads * a.tokens + 256 / LANES - 1) / (256 / LANES)), a.batch < 65535 ? a.batch : 65535);
+    if (format == DF11_KV_INT8) kv_append_kernel<LANES, DF11_KV_INT8, T><<<grid, 256, 0, stream>>>(a);
+    else kv_append_kernel<LANES, DF11_KV_E4M3, T><<<grid, 256, 0, stream>>>(a);
+}
+
+template <typename T> void launch_append(const AppendArgs &a, int format, cudaStream_t stream)
+{
+    if (a.dim <= 64) launch_append<4, T>(a, format, stream);
+    else if (a.dim <= 128) launch_append<8, T>(a, format, stream);
+    else launch_append<16, T>(a, format, stream);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -927,24 +1031,19 @@ extern "C" int df11_kv_append(const void *k, const void *v, int64_t k_stride_b, 
     if (((uintptr_t)k | (uintptr_t)v) & 1 || ((uintptr_t)positions & 7)) return df11_fail(DF11_ERR_BADARG, "misaligned pointer");
     if (n_positions != 1 && n_positions != batch) return df11_fail(DF11_ERR_BADARG, "positions must have 1 or batch entries");
     if (tokens < 0 || tokens > 0x7FFFFFFF) return df11_fail(DF11_ERR_BADARG, "bad token count");
-    const double all = 2.0 * (double)batch * kv_heads * (double)tokens;
-    if (all > 8e9) return df11_fail(DF11_ERR_BADARG, "too many rows for one call");
-    if (all == 0) return DF11_OK;
-    const int64_t rows = batch * kv_heads * tokens;
+    if (2.0 * kv_heads * (double)tokens > 2e9) return df11_fail(DF11_ERR_BADARG, "too many rows for one call");
+    if (batch == 0 || tokens == 0) return DF11_OK;
     Df11DeviceScope scope(device);
     if (!scope.ok) return df11_fail(DF11_ERR_CUDA, "cudaSetDevice(%d) failed", device);
-    const Strides ks = {k_stride_b, k_stride_h, k_stride_t}, vs = {v_stride_b, v_stride_h, v_stride_t};
-    const unsigned grid = (unsigned)((2 * rows + 3) / 4);
-    if (element_type == DF11_TYPE_BF16)
-        kv_append_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(
-            (const __nv_bfloat16 *)k, (const __nv_bfloat16 *)v, ks, vs, (uint8_t *)k_codes, (float *)k_scales, (uint8_t *)v_codes,
-            (float *)v_scales, (const int64_t *)positions, n_positions > 1, rows, kv_heads, tokens, head_dim, max_slots, format,
-            (int *)status);
-    else
-        kv_append_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(
-            (const __half *)k, (const __half *)v, ks, vs, (uint8_t *)k_codes, (float *)k_scales, (uint8_t *)v_codes,
-            (float *)v_scales, (const int64_t *)positions, n_positions > 1, rows, kv_heads, tokens, head_dim, max_slots, format,
-            (int *)status);
+    AppendArgs a = {};
+    a.k = k, a.v = v, a.ks = {k_stride_b, k_stride_h, k_stride_t}, a.vs = {v_stride_b, v_stride_h, v_stride_t};
+    a.k_codes = (uint8_t *)k_codes, a.v_codes = (uint8_t *)v_codes, a.k_scales = (float *)k_scales, a.v_scales = (float *)v_scales;
+    a.positions = (const int64_t *)positions, a.per_sequence = n_positions > 1, a.status = (int *)status;
+    a.max_slots = max_slots, a.batch = (uint32_t)batch, a.heads = (uint32_t)kv_heads, a.tokens = (uint32_t)tokens, a.dim = head_dim;
+    a.aligned = !((((uintptr_t)k | (uintptr_t)v) & 15) ||
+                  ((k_stride_b | k_stride_h | k_stride_t | v_stride_b | v_stride_h | v_stride_t) & 7));
+    if (element_type == DF11_TYPE_BF16) launch_append<__nv_bfloat16>(a, format, (cudaStream_t)stream);
+    else launch_append<__half>(a, format, (cudaStream_t)stream);
     return launched();
 }
 
@@ -959,21 +1058,19 @@ extern "C" int df11_kv_read(const void *k_codes, const void *k_scales, const voi
     if (((uintptr_t)k_out | (uintptr_t)v_out) & 15) return df11_fail(DF11_ERR_BADARG, "the results must be 16-byte aligned");
     if (first_slot < 0 || n_slots < 0 || first_slot > max_slots || n_slots > max_slots - first_slot)
         return df11_fail(DF11_ERR_BADARG, "slots %lld + %lld of %lld", (long long)first_slot, (long long)n_slots, (long long)max_slots);
-    const double all = 2.0 * (double)batch * kv_heads * (double)n_slots;
-    if (all > 8e9) return df11_fail(DF11_ERR_BADARG, "too many rows for one call");
-    if (all == 0) return DF11_OK;
-    const int64_t rows = batch * kv_heads * n_slots;
+    const int64_t units = batch * kv_heads, chunks = head_dim / 8, blocks = (n_slots * chunks + 1023) / 1024;
+    if (blocks > 0x7FFFFFFF || units > 0x7FFFFFFF) return df11_fail(DF11_ERR_BADARG, "too many slots for one call");
+    if (units == 0 || n_slots == 0) return DF11_OK;
     Df11DeviceScope scope(device);
     if (!scope.ok) return df11_fail(DF11_ERR_CUDA, "cudaSetDevice(%d) failed", device);
-    const unsigned grid = (unsigned)((2 * rows + 3) / 4);
-    if (element_type == DF11_TYPE_BF16)
-        kv_read_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(
-            (const uint8_t *)k_codes, (const float *)k_scales, (const uint8_t *)v_codes, (const float *)v_scales,
-            (__nv_bfloat16 *)k_out, (__nv_bfloat16 *)v_out, rows, max_slots, head_dim, first_slot, n_slots, format);
-    else
-        kv_read_kernel<<<grid, 128, 0, (cudaStream_t)stream>>>(
-            (const uint8_t *)k_codes, (const float *)k_scales, (const uint8_t *)v_codes, (const float *)v_scales,
-            (__half *)k_out, (__half *)v_out, rows, max_slots, head_dim, first_slot, n_slots, format);
+    ReadArgs a = {};
+    a.k_codes = (const uint8_t *)k_codes, a.v_codes = (const uint8_t *)v_codes, a.k_scales = (const float *)k_scales;
+    a.v_scales = (const float *)v_scales, a.k_out = k_out, a.v_out = v_out, a.max_slots = max_slots, a.first = first_slot;
+    a.units = (uint32_t)units, a.n = (uint32_t)n_slots, a.chunks = (uint32_t)chunks;
+    const dim3 grid((unsigned)blocks, (unsigned)(units < 65535 ? units : 65535), 2);
+    auto go = [&](auto kernel) { kernel<<<grid, 256, 0, (cudaStream_t)stream>>>(a); };
+    if (element_type == DF11_TYPE_BF16) format == DF11_KV_INT8 ? go(kv_read_kernel<DF11_KV_INT8, __nv_bfloat16>) : go(kv_read_kernel<DF11_KV_E4M3, __nv_bfloat16>);
+    else format == DF11_KV_INT8 ? go(kv_read_kernel<DF11_KV_INT8, __half>) : go(kv_read_kernel<DF11_KV_E4M3, __half>);
     return launched();
 }
 
