@@ -929,10 +929,10 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
 }
 
 template <typename K> cudaError_t launch_wide(K kernel, unsigned grid, unsigned block, size_t shared, unsigned cluster,
-                                              cudaStream_t stream, const AttentionArgs &a)
+                                              int device, cudaStream_t stream, const AttentionArgs &a)
 {
     if (shared > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        const cudaError_t e = df11_allow_shared((const void *)kernel, shared, device);
         if (e != cudaSuccess) return e;
     }
     cudaLaunchConfig_t config = {};
@@ -949,16 +949,16 @@ template <typename K> cudaError_t launch_wide(K kernel, unsigned grid, unsigned 
 }
 
 template <int D, int NT, int FMT, bool EXACT, typename T>
-cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStream_t stream)
+cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int device, cudaStream_t stream)
 {
     constexpr int kRows = NT * 8;
     constexpr size_t kJoin = (size_t)(kAttWarps * kRows * D + 2 * kAttWarps * kRows + 2 * kRows) * sizeof(float);
     constexpr size_t kRing = (size_t)kAttWarps * kAttStages<D> * (32 * D + 128), kShared = kRing > kJoin ? kRing : kJoin;
     if (d.cluster)
         return launch_wide(kv_attention_kernel<D, NT, FMT, EXACT, T>, (unsigned)d.ctas, kAttWarps * 32, kShared, (unsigned)d.cluster,
-                           stream, a);
+                           device, stream, a);
     const cudaError_t e = launch_wide(kv_attention_shared_kernel<D, NT, FMT, EXACT, T>, (unsigned)d.ctas, kAttWarps * 32, kShared, 1,
-                                      stream, a);
+                                      device, stream, a);
     if (e != cudaSuccess) return e;
     // the joining kernel is launched while the first still runs and waits for its end on the device
     cudaLaunchConfig_t config = {};
@@ -973,15 +973,15 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, cudaStre
     return cudaLaunchKernelEx(&config, kv_attention_join_kernel<D, NT, T>, a, (uint32_t)d.ctas);
 }
 
-template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, cudaStream_t stream)
+template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, int device, cudaStream_t stream)
 {
 #define DF11_ATTENTION(D, NT)                                                                             \
     if (d.width == D && d.tiles_n == NT) {                                                                \
         if (format == DF11_KV_INT8)                                                                       \
-            return a.dim == D ? launch_attention<D, NT, DF11_KV_INT8, true, T>(a, d, stream)              \
-                              : launch_attention<D, NT, DF11_KV_INT8, false, T>(a, d, stream);            \
-        return a.dim == D ? launch_attention<D, NT, DF11_KV_E4M3, true, T>(a, d, stream)                  \
-                          : launch_attention<D, NT, DF11_KV_E4M3, false, T>(a, d, stream);                \
+            return a.dim == D ? launch_attention<D, NT, DF11_KV_INT8, true, T>(a, d, device, stream)              \
+                              : launch_attention<D, NT, DF11_KV_INT8, false, T>(a, d, device, stream);            \
+        return a.dim == D ? launch_attention<D, NT, DF11_KV_E4M3, true, T>(a, d, device, stream)                  \
+                          : launch_attention<D, NT, DF11_KV_E4M3, false, T>(a, d, device, stream);                \
     }
     DF11_ATTENTION(64, 1)
     DF11_ATTENTION(64, 2)
@@ -1123,8 +1123,8 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     a.kv_heads = (uint32_t)kv_heads, a.group = (uint32_t)(heads / kv_heads), a.dim = head_dim, a.window = window;
     a.batch = (uint32_t)batch, a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster;
     a.queries = (uint32_t)queries, a.max_slots = max_slots, a.scale = scale;
-    const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, (cudaStream_t)stream)
-                                                         : launch_attention<__half>(a, d, format, (cudaStream_t)stream);
+    const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, device, (cudaStream_t)stream)
+                                                         : launch_attention<__half>(a, d, format, device, (cudaStream_t)stream);
     if (e != cudaSuccess) return df11_fail(DF11_ERR_CUDA, "kernel launch failed: %s", cudaGetErrorString(e));
     return DF11_OK;
 }

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/df11.h"
 #include "df11_error.h"
 
@@ -25,6 +27,20 @@ struct Df11DeviceScope {
     Df11DeviceScope(const Df11DeviceScope &) = delete;
     Df11DeviceScope &operator=(const Df11DeviceScope &) = delete;
 };
+
+// Lets `kernel` use `bytes` of shared memory on the current device, which is `device`.  The runtime is asked once per
+// kernel and device: the answer stays, and asking costs as much as a launch's other bookkeeping together.
+inline cudaError_t df11_allow_shared(const void *kernel, size_t bytes, int device)
+{
+    constexpr int kPlaces = 256;
+    static std::atomic<const void *> known[kPlaces];
+    const size_t at = ((reinterpret_cast<uintptr_t>(kernel) >> 3) + (size_t)device * 61) % kPlaces;
+    const void *const tag = reinterpret_cast<const char *>(kernel) + (device & 7);
+    if (device < 8 && known[at].load(std::memory_order_relaxed) == tag) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 8) known[at].store(tag, std::memory_order_relaxed);
+    return e;
+}
 
 template <typename T> __device__ __forceinline__ float df11_to_float(T x);
 template <> __device__ __forceinline__ float df11_to_float<float>(float x) { return x; }

@@ -853,7 +853,7 @@ extern "C" int df11_sample(const void *logits, int64_t row_stride, int32_t eleme
     a.temperature_value = temperature_value, a.top_p_value = top_p_value, a.min_p_value = min_p_value, a.top_k_value = top_k_value;
     a.out = (int64_t *)out, a.status = (int *)status;
     auto go = [&](auto kernel) {
-        const cudaError_t set = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Shared));
+        const cudaError_t set = df11_allow_shared((const void *)kernel, sizeof(Shared), device);
         if (set != cudaSuccess) return set;
         cudaLaunchConfig_t config = {};
         config.gridDim = dim3((unsigned)(rows * cluster));

@@ -219,7 +219,12 @@ def gemv_prepared(luts: torch.Tensor, encoded_exponent: torch.Tensor, sign_manti
 
 
 # ------------------------------------------------------------------ operators of a generation step
+#
+# A single-token step launches these once per layer, so the host time of a call counts: each first asks in one
+# expression whether everything is as it should be (some 3 microseconds), and only if not goes through the checks
+# one by one, which name what is wrong.
 _ELEMENT_TYPES = {torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_FP16, torch.float32: _lib.TYPE_FP32}
+_LEAST, _MOST = 5e-324, 1.7976931348623157e308
 KV_FORMATS = {torch.int8: _lib.KV_INT8, torch.float8_e4m3fn: _lib.KV_E4M3}
 
 
@@ -255,6 +260,27 @@ def _cache(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor,
     return (device, KV_FORMATS[k_codes.dtype], *k_codes.shape)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream_at(index: int) -> int:
+    """The current stream of CUDA device ``index``, without making a stream object where torch allows it."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _cache_fits(at: int, k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, shape) -> bool:
+    dtype, rows = k_codes.dtype, shape[:3]
+    return (at >= 0 and len(shape) == 4 and dtype in KV_FORMATS and v_codes.dtype == dtype and v_codes.shape == shape
+            and k_scales.shape == rows and v_scales.shape == rows and k_scales.dtype == torch.float32
+            and v_scales.dtype == torch.float32 and v_codes.get_device() == at and k_scales.get_device() == at
+            and v_scales.get_device() == at and k_codes.is_contiguous() and v_codes.is_contiguous()
+            and k_scales.is_contiguous() and v_scales.is_contiguous())
+
+
+def _indices_fit(at: int, t: torch.Tensor, batch: int) -> bool:
+    return t.get_device() == at and t.dtype == torch.int64 and t.is_contiguous() and t.numel() in (1, batch)
+
+
 def _per_sequence(name: str, t: torch.Tensor, batch: int, device: torch.device) -> torch.Tensor:
     _require_cuda(**{name: t})
     if t.device != device:
@@ -275,20 +301,31 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales:
     and stands for ``code * scale``, with the code nearest to ``x / scale`` (ties to even); a row with an infinity or
     a NaN stands for NaNs.  ``positions``: int64, one per sequence or one for all.  Tokens whose slot the cache does not
     have are left out and set ``STATUS_BAD_POSITIONS`` in ``status``."""
-    device, fmt, batch, heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
-    _activation("k", k, (batch, heads, None, dim), device)
-    _activation("v", v, (batch, heads, k.shape[2], dim), device)
-    if v.dtype != k.dtype:
-        raise RuntimeError("`k` and `v` must have one dtype")
-    _per_sequence("positions", positions, batch, device)
-    _require_cuda(k_codes=k_codes, status=status)
+    shape, at = k_codes.shape, k_codes.get_device()
+    if not (_cache_fits(at, k_codes, k_scales, v_codes, v_scales, shape) and _indices_fit(at, positions, shape[0])
+            and k.get_device() == at and v.get_device() == at and k.shape == v.shape and k.dim() == 4
+            and k.shape[:2] == shape[:2] and k.shape[3] == shape[3] and (k.dtype == torch.bfloat16 or k.dtype == torch.float16)
+            and v.dtype == k.dtype and not (k.requires_grad or v.requires_grad) and status is None
+            and k.stride(3) == 1 and v.stride(3) == 1):
+        device, _, batch, heads, _, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+        _activation("k", k, (batch, heads, None, dim), device)
+        _activation("v", v, (batch, heads, k.shape[2], dim), device)
+        if v.dtype != k.dtype:
+            raise RuntimeError("`k` and `v` must have one dtype")
+        _per_sequence("positions", positions, batch, device)
+        _require_cuda(k_codes=k_codes, status=status)
+    batch, heads, slots, dim = shape
+    tokens = k.shape[2]
     if not k.numel():
         return
-    _lib.check(_lib.lib.df11_kv_append(
-        k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], k_codes.data_ptr(), k_scales.data_ptr(),
-        v_codes.data_ptr(), v_scales.data_ptr(), positions.data_ptr(), positions.numel(), batch, heads, k.shape[2], dim,
-        slots, _ELEMENT_TYPES[k.dtype], fmt, status.data_ptr() if status is not None else None, device.index,
-        _stream(device)))
+    ks, vs = k.stride(), v.stride()
+    rc = _lib.lib.df11_kv_append(
+        k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], k_codes.data_ptr(), k_scales.data_ptr(),
+        v_codes.data_ptr(), v_scales.data_ptr(), positions.data_ptr(), positions.numel(), batch, heads, tokens, dim,
+        slots, _ELEMENT_TYPES[k.dtype], KV_FORMATS[k_codes.dtype], status.data_ptr() if status is not None else None, at,
+        _stream_at(at))
+    if rc:
+        _lib.check(rc)
 
 
 def kv_read(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor, v_scales: torch.Tensor, first_slot: int,
@@ -296,7 +333,10 @@ def kv_read(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor
     """Slots ``[first_slot, first_slot + n_slots)`` of every sequence as ``(k, v)``, each
     ``[batch, kv_heads, n_slots, head_dim]`` in ``dtype`` (BF16 or FP16): ``code * scale`` in fp32, rounded once.
     ``out`` may hold the two contiguous tensors to fill."""
-    device, fmt, batch, heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+    cache, at = k_codes.shape, k_codes.get_device()
+    if not _cache_fits(at, k_codes, k_scales, v_codes, v_scales, cache):
+        _cache(k_codes, k_scales, v_codes, v_scales)
+    batch, heads, slots, dim = cache
     if dtype not in (torch.bfloat16, torch.float16):
         raise RuntimeError(f"`dtype` must be bfloat16 or float16, not {dtype}")
     first_slot, n_slots = int(first_slot), int(n_slots)
@@ -304,16 +344,20 @@ def kv_read(k_codes: torch.Tensor, k_scales: torch.Tensor, v_codes: torch.Tensor
         raise RuntimeError(f"slots {first_slot} .. {first_slot + n_slots} are not in a cache of {slots}")
     shape = (batch, heads, n_slots, dim)
     if out is None:
-        k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+        k = torch.empty(shape, dtype=dtype, device=k_codes.device)
+        v = torch.empty(shape, dtype=dtype, device=k_codes.device)
     else:
         k, v = out
         _require_cuda(k_codes=k_codes, k=k, v=v)
         if any(t.dtype != dtype or tuple(t.shape) != shape for t in (k, v)):
             raise RuntimeError(f"`out` must be two {dtype} tensors of shape {shape}")
     if k.numel():
-        _lib.check(_lib.lib.df11_kv_read(
+        rc = _lib.lib.df11_kv_read(
             k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), k.data_ptr(), v.data_ptr(),
-            batch, heads, slots, dim, first_slot, n_slots, _ELEMENT_TYPES[dtype], fmt, device.index, _stream(device)))
+            batch, heads, slots, dim, first_slot, n_slots, _ELEMENT_TYPES[dtype], KV_FORMATS[k_codes.dtype], at,
+            _stream_at(at))
+        if rc:
+            _lib.check(rc)
     return k, v
 
 
@@ -331,31 +375,44 @@ def kv_attention(q: torch.Tensor, k_codes: torch.Tensor, k_scales: torch.Tensor,
     follows wants it; a query that sees nothing gives zeros.  Any number of queries works; what the kernel is made for
     is one to some sixteen rows per key head (a long prompt is better read back with ``kv_read``).
     Working memory is allocated per call, so calls may overlap on different streams."""
-    device, fmt, batch, kv_heads, slots, dim = _cache(k_codes, k_scales, v_codes, v_scales)
-    _activation("q", q, (batch, None, None, dim), device)
-    heads, queries = q.shape[1], q.shape[2]
+    cache, at, shape = k_codes.shape, k_codes.get_device(), q.shape
+    if not (_cache_fits(at, k_codes, k_scales, v_codes, v_scales, cache) and _indices_fit(at, lengths, cache[0])
+            and (first is None or _indices_fit(at, first, cache[0])) and q.get_device() == at and len(shape) == 4
+            and shape[0] == cache[0] and shape[3] == cache[3] and (q.dtype == torch.bfloat16 or q.dtype == torch.float16)
+            and not q.requires_grad and q.stride(3) == 1):
+        device, _, batch, _, _, dim = _cache(k_codes, k_scales, v_codes, v_scales)
+        _activation("q", q, (batch, None, None, dim), device)
+        _per_sequence("lengths", lengths, batch, device)
+        if first is not None:
+            _per_sequence("first", first, batch, device)
+    batch, kv_heads, slots, dim = cache
+    heads, queries = shape[1], shape[2]
     if heads < 1 or heads % kv_heads:
         raise RuntimeError(f"{heads} query heads on {kv_heads} key heads")
-    _per_sequence("lengths", lengths, batch, device)
-    if first is not None:
-        _per_sequence("first", first, batch, device)
+    window = int(window)
     if window < 0:
         raise RuntimeError("`window` must not be negative")
     if out is None:
-        out = torch.empty(batch, queries, heads, dim, dtype=q.dtype, device=device)
-    _require_cuda(k_codes=k_codes, out=out)
-    if out.dtype != q.dtype or tuple(out.shape) != (batch, queries, heads, dim):
-        raise RuntimeError(f"`out` must be a {q.dtype} tensor of shape {(batch, queries, heads, dim)}")
+        out = torch.empty((batch, queries, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _require_cuda(k_codes=k_codes, out=out)
+        if out.dtype != q.dtype or tuple(out.shape) != (batch, queries, heads, dim):
+            raise RuntimeError(f"`out` must be a {q.dtype} tensor of shape {(batch, queries, heads, dim)}")
     if not q.numel():
         return out
-    need = _lib.check(_lib.lib.df11_kv_attention_workspace_bytes(batch, heads, kv_heads, queries, dim, slots, int(window)))
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _lib.check(_lib.lib.df11_kv_attention(
-        q.data_ptr(), *q.stride()[:3], k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
+    need = _lib.lib.df11_kv_attention_workspace_bytes(batch, heads, kv_heads, queries, dim, slots, window)
+    if need < 0:
+        _lib.check(need)
+    workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    qs = q.stride()
+    rc = _lib.lib.df11_kv_attention(
+        q.data_ptr(), qs[0], qs[1], qs[2], k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(),
         lengths.data_ptr(), lengths.numel(), first.data_ptr() if first is not None else None,
         first.numel() if first is not None else 0, out.data_ptr(), workspace.data_ptr() if need else None, need, batch,
-        heads, kv_heads, queries, dim, slots, int(window), dim ** -0.5 if scale is None else float(scale),
-        _ELEMENT_TYPES[q.dtype], fmt, device.index, _stream(device)))
+        heads, kv_heads, queries, dim, slots, window, dim ** -0.5 if scale is None else scale,
+        _ELEMENT_TYPES[q.dtype], KV_FORMATS[k_codes.dtype], at, _stream_at(at))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -372,35 +429,41 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
     gives 0 and sets ``STATUS_EMPTY_ROW`` in ``status``."""
     if not logits.is_cuda:
         raise RuntimeError(f"df11 kernels need CUDA tensors; `logits` is on {logits.device}")
-    device = logits.device
     if logits.dim() != 2 or logits.shape[1] < 1 or logits.dtype not in _ELEMENT_TYPES:
         raise RuntimeError("`logits` must be [rows, vocab] in bfloat16, float16 or float32")
-    rows, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    at, (rows, vocab) = logits.get_device(), logits.shape
+    stride = logits.stride()
+    if vocab > 1 and stride[1] != 1:
         raise RuntimeError("the rows of `logits` must be contiguous")
+
+    def fits(t, dtype):
+        return t.get_device() == at and t.dtype == dtype and t.numel() == rows and t.is_contiguous()
+
+    if not fits(uniform, torch.float32):
+        raise RuntimeError(f"`uniform` must be a contiguous float32 tensor of {rows} elements on {logits.device}")
     if out is None:
-        out = torch.empty(rows, dtype=torch.int64, device=device)
-    _require_cuda(uniform=uniform, out=out, status=status)
-    if uniform.device != device or uniform.dtype != torch.float32 or uniform.numel() != rows:
-        raise RuntimeError(f"`uniform` must be a float32 tensor of {rows} elements on {device}")
-    if out.device != device or out.dtype != torch.int64 or out.numel() != rows:
-        raise RuntimeError(f"`out` must be an int64 tensor of {rows} elements on {device}")
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    elif not fits(out, torch.int64):
+        raise RuntimeError(f"`out` must be a contiguous int64 tensor of {rows} elements on {logits.device}")
+    if status is not None:
+        _require_cuda(out=out, status=status)
     args = []
-    for name, value, dtype, fits in (("temperature", temperature, torch.float32, lambda x: 0 <= x < float("inf")),
-                                     ("top_k", top_k, torch.int32, lambda x: 0 <= x < 2 ** 31),
-                                     ("top_p", top_p, torch.float32, lambda x: 0 < x <= 1),
-                                     ("min_p", min_p, torch.float32, lambda x: 0 <= x <= 1)):
+    for name, value, dtype, low, high in (("temperature", temperature, torch.float32, 0, _MOST), ("top_k", top_k, torch.int32, 0, 2 ** 31 - 1),
+                                          ("top_p", top_p, torch.float32, _LEAST, 1), ("min_p", min_p, torch.float32, 0, 1)):
         if isinstance(value, torch.Tensor):
-            _require_cuda(**{name: value})
-            if value.device != device or value.dtype != dtype or value.numel() != rows:
-                raise RuntimeError(f"`{name}` must be a number or a {dtype} tensor of {rows} elements on {device}")
-            args += [value.data_ptr(), 0]
+            if not fits(value, dtype):
+                raise RuntimeError(f"`{name}` must be a number or a contiguous {dtype} tensor of {rows} elements on {logits.device}")
+            args.append(value.data_ptr())
+            args.append(0)
         else:
-            if not fits(value):
+            if not low <= value <= high:
                 raise RuntimeError(f"`{name}` = {value} is out of range")
-            args += [None, int(value) if dtype == torch.int32 else float(value)]
+            args.append(None)
+            args.append(int(value) if name == "top_k" else float(value))
     if rows:
-        _lib.check(_lib.lib.df11_sample(
-            logits.data_ptr(), logits.stride(0), _ELEMENT_TYPES[logits.dtype], rows, vocab, uniform.data_ptr(), *args,
-            out.data_ptr(), status.data_ptr() if status is not None else None, device.index, _stream(device)))
+        rc = _lib.lib.df11_sample(
+            logits.data_ptr(), stride[0], _ELEMENT_TYPES[logits.dtype], rows, vocab, uniform.data_ptr(), *args,
+            out.data_ptr(), status.data_ptr() if status is not None else None, at, _stream_at(at))
+        if rc:
+            _lib.check(rc)
     return out
