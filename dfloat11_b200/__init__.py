@@ -9,6 +9,7 @@ from .dfloat11 import (DFloat11Model, TensorManager, check_status, compress_in_p
                        get_no_split_classes, load_and_replace_tensors, stats)
 from . import ops  # noqa: F401
 from .generation import GraphedGreedyDecoder
+from .kv_cache import QuantizedKVCache
 from .ops import (aux_bytes, decode, decode_prepared, decode_range_prepared, decode_rows_prepared, gemv_prepared,
                   kv_append, kv_attention, kv_read, prepare, sample, seek_interval)
 
@@ -18,5 +19,5 @@ __all__ = [
     "UnrepresentableError", "encode_weights", "get_codec", "get_luts", "split_bf16", "validate_unit",
     "aux_bytes", "decode", "decode_prepared", "decode_range_prepared", "decode_rows_prepared", "gemv_prepared",
     "prepare", "seek_interval", "ops", "kv_append", "kv_attention", "kv_read", "sample",
-    "GraphedGreedyDecoder",
+    "GraphedGreedyDecoder", "QuantizedKVCache",
 ]

@@ -173,7 +173,8 @@ def check_status(reset: bool = True) -> None:
     up waiting for a peer.  Synchronises with the devices, so it is not called per forward unless
     ``DF11_CHECK_STATUS=1`` is set."""
     names = {_lib.STATUS_BAD_TABLE: "bad table", _lib.STATUS_BAD_POSITIONS: "bad positions or index",
-             _lib.STATUS_TRUNCATED: "truncated block", _lib.STATUS_TIMEOUT: "copy timed out"}
+             _lib.STATUS_TRUNCATED: "truncated block", _lib.STATUS_TIMEOUT: "copy timed out",
+             _lib.STATUS_EMPTY_ROW: "logits with nothing to draw from"}
     for device, word in _status_words.items():
         bits = int(word.item())
         if bits:

@@ -305,7 +305,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales:
     if not (_cache_fits(at, k_codes, k_scales, v_codes, v_scales, shape) and _indices_fit(at, positions, shape[0])
             and k.get_device() == at and v.get_device() == at and k.shape == v.shape and k.dim() == 4
             and k.shape[:2] == shape[:2] and k.shape[3] == shape[3] and (k.dtype == torch.bfloat16 or k.dtype == torch.float16)
-            and v.dtype == k.dtype and not (k.requires_grad or v.requires_grad) and status is None
+            and v.dtype == k.dtype and not (k.requires_grad or v.requires_grad)
+            and (status is None or (status.get_device() == at and status.dtype == torch.int32))
             and k.stride(3) == 1 and v.stride(3) == 1):
         device, _, batch, heads, _, dim = _cache(k_codes, k_scales, v_codes, v_scales)
         _activation("k", k, (batch, heads, None, dim), device)
@@ -314,6 +315,8 @@ def kv_append(k: torch.Tensor, v: torch.Tensor, k_codes: torch.Tensor, k_scales:
             raise RuntimeError("`k` and `v` must have one dtype")
         _per_sequence("positions", positions, batch, device)
         _require_cuda(k_codes=k_codes, status=status)
+        if status is not None and status.dtype != torch.int32:
+            raise RuntimeError("`status` must be an int32 tensor")
     batch, heads, slots, dim = shape
     tokens = k.shape[2]
     if not k.numel():
@@ -445,8 +448,8 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
         out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     elif not fits(out, torch.int64):
         raise RuntimeError(f"`out` must be a contiguous int64 tensor of {rows} elements on {logits.device}")
-    if status is not None:
-        _require_cuda(out=out, status=status)
+    if status is not None and (status.get_device() != at or status.dtype != torch.int32):
+        raise RuntimeError(f"`status` must be an int32 tensor on {logits.device}")
     args = []
     for name, value, dtype, low, high in (("temperature", temperature, torch.float32, 0, _MOST), ("top_k", top_k, torch.int32, 0, 2 ** 31 - 1),
                                           ("top_p", top_p, torch.float32, _LEAST, 1), ("min_p", min_p, torch.float32, 0, 1)):
