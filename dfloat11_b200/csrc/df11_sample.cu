@@ -62,42 +62,52 @@ __device__ __forceinline__ float logit_of(uint32_t key)
 constexpr int kRoots = 32;
 constexpr double kOne52 = 4503599627370496.0;  // 2^52: added to a number below it, the sum's low bits are the nearest integer
 struct Weigher {
-    float best, cap, cut;                     // cut: below, a weight is less than 2^-60 and taken as 0
+    float cap, cut;                           // the largest logit that counts, and one below which a weight is less than 2^-60
+    bool plain;                               // -inf gets no weight by itself; otherwise the caller must not ask
     double peak, slope, unit;
     int shift;                                // S
     const double *roots;                      // 2^(j/32), in shared memory
 
-    __device__ __forceinline__ Weigher(float b, double t, int s, const double *r) : best(b), shift(s), roots(r)
+    __device__ __forceinline__ Weigher(float best, double t, int s, const double *r) : shift(s), roots(r)
     {
-        const double inverse = fmin(1.0 / t, 1e300);
-        cap = b == INFINITY ? 0.0f : b;       // beside a +inf only its like have a weight
-        cut = b == INFINITY ? b : fmaxf((float)(b - 60.0 * 0.69314718055994530942 * t), -3.402823466e38f);
+        constexpr float kMost = 3.402823466e38f;
+        cap = fminf(best, kMost);
+        const float low = (float)fmax(cap - 60.0 * 0.69314718055994530942 * t, -(double)kMost);
+        plain = best <= kMost && low > -kMost;
+        cut = low > -kMost ? logit_of(key_of(low) - 1) : low;     // rounded down
         peak = (double)cap;
-        slope = inverse * (kRoots * 1.4426950408889634074);
+        // the second where even the float below the largest is thousands of octaves away
+        slope = fmin(kRoots * 1.4426950408889634074 / t, 0x1p30 / (peak - (double)cut));
         unit = ldexp(1.0, s);
     }
-    // 0 for a NaN and for -inf; exactly 2^S for the largest
+    // exactly 2^S for the largest; less than 1/2 for what is below `cut`, -inf included
     __device__ __forceinline__ double real(float z) const
     {
         constexpr double kMagic = 1.5 * kOne52;
         constexpr double a = 0.69314718055994530942 / kRoots;
-        const bool some = z >= cut;
-        const double t = ((double)fminf(some ? z : best, cap) - peak) * slope;
+        const double t = ((double)fminf(fmaxf(z, cut), cap) - peak) * slope;
         const double m = t + kMagic;
-        const int n = __double2loint(m);
+        const int n = max(__double2loint(m), -63 * kRoots);
         const double f = t - (m - kMagic);
         double p = fma(a * a * a * a * a / 120, f, a * a * a * a / 24);
         p = fma(p, f, a * a * a / 6);
         p = fma(p, f, a * a / 2);
         p = fma(p, f, a);
         const double root = roots[n & (kRoots - 1)];
-        const double scaled = __hiloint2double(__double2hiint(root) + (((n >> 5) + shift) << 20), __double2loint(root));
-        return some ? fma(scaled, p * f, scaled) : 0.0;
+        const double scaled = __hiloint2double(__double2hiint(root) + (n & -kRoots) * (1 << 15) + (shift << 20), __double2loint(root));
+        return fma(scaled, p * f, scaled);
     }
     // The nearest integer to w < 2^51, plus kBias; sums of such numbers are put right by as many kBias.
     static constexpr u64 kBias = 0x4330000000000000ull;
     __device__ __forceinline__ static u64 biased(double w) { return (u64)__double_as_longlong(w + kOne52); }
     __device__ __forceinline__ u64 operator()(float z) const { return biased(real(z)) - kBias; }
+};
+
+struct Yes {
+    static constexpr bool value = true;
+};
+struct No {
+    static constexpr bool value = false;
 };
 
 struct Row {             // settings of a row
@@ -554,7 +564,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
         // tokens per interval
         const float range = fminf(best - fmaxf(least, lowest), 31.2f * (float)fmin(row.t, 1e37));
         const float scale = range > 0.0f ? fminf((float)kBins / range, 1e30f) : 0.0f;
-        auto bin_of = [&](float z) { return z == best ? 0 : (int)fminf((best - z) * scale, (float)(kBins - 1)); };
+        // An interval's number, as the low bits of a float.  Beside a +inf all that counts is equal.
+        constexpr float kMagic = 8388608.0f;
+        const float from = fminf(best, 3.402823466e38f);
+        auto place_of = [&](float z) { return fminf(fmaf(from - z, scale, kMagic), kMagic + (kBins - 1)); };
+        auto bin_of = [&](float z) { return (int)(__float_as_uint(place_of(fminf(z, from))) & (kBins - 1)); };
         for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
         __syncthreads();
 #pragma unroll 2
@@ -675,39 +689,45 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             }
             __syncthreads();
             // one pass: mass of what top-k keeps, mass above the intervals, sums of blocks of the latter
-            const float low = (float)s.bin_low, high = s.bin_high == kBins - 1 ? INFINITY : (float)(s.bin_high + 1);
+            const float low = kMagic + s.bin_low, high = kMagic + s.bin_high;
             u64 mass_all = 0, mass_above = 0;
-            for (uint32_t block = warp; block < blocks; block += kWarps) {
-                u64 part = 0;
-                for (int x = 0; x < 1 << wide; ++x) {
-                    const uint32_t g = g0 + block * block_groups + x * 32 + lane, index = g * 8 - tokens.lead;
-                    if (g >= g1) continue;
-                    float z[8];
-                    tokens.logits(g, z);
-                    uint32_t on_list = 0;
+            auto add_up = [&](auto ranked, auto floored) {
+                for (uint32_t block = warp; block < blocks; block += kWarps) {
+                    u64 part = 0;
+                    for (int x = 0; x < 1 << wide; ++x) {
+                        const uint32_t g = g0 + block * block_groups + x * 32 + lane, index = g * 8 - tokens.lead;
+                        if (g >= g1) continue;
+                        float z[8];
+                        tokens.logits(g, z);
+                        uint32_t on_list = 0;
+                        u64 above = 0;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const bool kept = is_kept(z[j], index + j);
-                        const float interval = z[j] == best ? 0.0f : (best - z[j]) * scale;
-                        const bool over = kept && interval < low;
-                        const double w = weigh.real(z[j]);
-                        const u64 all = weigh.biased(kept ? w : 0.0);
-                        mass_all += all;
-                        mass_above += over ? all : weigh.kBias;
-                        part += over && w >= floor ? all : weigh.kBias;
-                        if (kept && !over && interval < high) on_list |= 1u << j;
-                    }
-                    mass_all -= 8 * weigh.kBias, mass_above -= 8 * weigh.kBias, part -= 8 * weigh.kBias;
-                    if (on_list) {
+                        for (int j = 0; j < 8; ++j) {
+                            const bool kept = !ranked.value || is_kept(z[j], index + j);
+                            const float place = place_of(ranked.value ? fminf(z[j], from) : z[j]);
+                            const double w = weigh.real(z[j]);
+                            const u64 all = weigh.biased(kept ? w : 0.0);
+                            mass_all += all;
+                            above += place < low ? all : weigh.kBias;
+                            if (floored.value) part += place < low && w >= floor ? all : weigh.kBias;
+                            if (place >= low && place <= high && kept && z[j] >= lowest) on_list |= 1u << j;
+                        }
+                        mass_all -= 8 * weigh.kBias, above -= 8 * weigh.kBias;
+                        mass_above += above;
+                        part += floored.value ? 0 - 8 * weigh.kBias : above;
+                        if (on_list) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (on_list >> j & 1) list_token(z[j], index + j);
+                            for (int j = 0; j < 8; ++j)
+                                if (on_list >> j & 1) list_token(z[j], index + j);
+                        }
                     }
+#pragma unroll
+                    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+                    if (lane == 0) s.blocks[block] = part;
                 }
-#pragma unroll
-                for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-                if (lane == 0) s.blocks[block] = part;
-            }
+            };
+            if (!by_rank && weigh.plain) floor > 0.0 ? add_up(No{}, Yes{}) : add_up(No{}, No{});
+            else floor > 0.0 ? add_up(Yes{}, Yes{}) : add_up(Yes{}, No{});
             mass_all = block_sum(mass_all, s.partial);
             mass_above = block_sum(mass_above, s.partial);
             if (tid == 0) s.mine.mass = mass_all, s.mine.above = mass_above;
@@ -748,24 +768,28 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
         }
     }
     if (!by_mass) {
-        for (uint32_t block = warp; block < blocks; block += kWarps) {
-            u64 part = 0;
-            for (int x = 0; x < 1 << wide; ++x) {
-                const uint32_t g = g0 + block * block_groups + x * 32 + lane;
-                if (g >= g1) continue;
-                float z[8];
-                tokens.logits(g, z);
+        auto add_up = [&](auto filtered) {
+            for (uint32_t block = warp; block < blocks; block += kWarps) {
+                u64 part = 0;
+                for (int x = 0; x < 1 << wide; ++x) {
+                    const uint32_t g = g0 + block * block_groups + x * 32 + lane;
+                    if (g >= g1) continue;
+                    float z[8];
+                    tokens.logits(g, z);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const double w = weigh.real(z[j]);
-                    part += weigh.biased(is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor ? w : 0.0);
+                    for (int j = 0; j < 8; ++j) {
+                        const double w = weigh.real(z[j]);
+                        part += weigh.biased(!filtered.value || (is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor) ? w : 0.0);
+                    }
+                    part -= 8 * weigh.kBias;
                 }
-                part -= 8 * weigh.kBias;
-            }
 #pragma unroll
-            for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-            if (lane == 0) s.blocks[block] = part;
-        }
+                for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+                if (lane == 0) s.blocks[block] = part;
+            }
+        };
+        if (by_rank || floor > 0.0 || !weigh.plain) add_up(Yes{});
+        else add_up(No{});
     }
     // the draw: the CTA, the block, the token
     __syncthreads();

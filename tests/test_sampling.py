@@ -170,7 +170,7 @@ def test_last_position_of_a_sequence_of_logits():
 @gpu
 def test_extreme_temperatures():
     logits, uniform = rows_of(6, 2003, torch.float32, seed=9)
-    for t in (1e-38, 1e-6, 1e6, 3e38):
+    for t in (1e-38, 1e-9, 3e-8, 1e-7, 1e-6, 1e6, 1e30, 1e37, 3e38):
         check(logits, uniform, temperature=t)
         check(logits, uniform, temperature=torch.full((6,), t, device=DEV), top_p=0.7)
     greedy = ops.sample(logits, uniform, temperature=0.0)
@@ -178,6 +178,26 @@ def test_extreme_temperatures():
         assert torch.equal(ops.sample(logits, uniform, temperature=torch.full((6,), t, device=DEV)), greedy)
     for p in (0.0, -1.0):
         assert torch.equal(ops.sample(logits, uniform, top_p=torch.full((6,), p, device=DEV)), greedy)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [1e-7, 1e-6, 1e-5, 1.0, 1e36, 1e37, 3e38])
+def test_neighbouring_and_outermost_logits(temperature):
+    """Logits one float apart (a temperature of their spacing tells them apart), and the type's ends, beside -inf."""
+    z = torch.full((4, 3000), float("-inf"))
+    near = torch.tensor([10.0]).repeat(40)
+    for i in range(1, 40):
+        near[i] = torch.nextafter(near[i - 1], torch.tensor(0.0))
+    z[0, 100:140] = near
+    z[1, ::50] = torch.finfo(torch.float32).max
+    z[1, 7] = torch.finfo(torch.float32).min
+    z[2, ::70] = torch.finfo(torch.float32).min
+    z[3, ::3] = torch.finfo(torch.float32).min
+    z[3, 5], z[3, 9] = 0.0, torch.finfo(torch.float32).max
+    z = z.to(DEV)
+    for u in (0.1, 0.5, 0.93):
+        for settings in ({}, dict(top_p=0.6), dict(min_p=0.3), dict(top_k=300, top_p=0.9), dict(top_k=5)):
+            check(z, torch.full((4,), u, device=DEV), temperature=temperature, **settings)
 
 
 @gpu
