@@ -11,13 +11,13 @@
 // A filter keeps all tokens above some logit and, of those equal to it, the ones up to some index.
 // That border is found without sorting the row:
 //   * top-k of a few: the k-th largest of the threads' own largest logits is a lower bound of the k-th
-//     largest of all.  The tokens above it are few; they are listed, sorted, and all filters and the
-//     draw are done on the list.
+//     largest of all.  The tokens above it are few; they are listed, and all filters and the draw are
+//     done on the list.
 //   * otherwise the tokens are counted in 4096 intervals of equal width between the largest logit
 //     and the one whose weight no longer matters (or the smallest).  Counts give the interval of the top-k border
 //     exactly, and, times the weight in the interval's middle, that of the top-p border almost.
 //     One pass over the row then adds up the exact mass above those intervals and lists what lies in them;
-//     the sorted list gives the border, and exact sums prove that it lies there.
+//     the list gives the border, and exact sums prove that it lies there.
 //   * where a list would overflow (thousands of equal logits at the border) or the guess was
 //     wrong, one CTA finds the border digit by digit of the logits' bits.
 // The draw needs masses in index order: sums of blocks of 256 or more tokens are kept by the same
@@ -25,7 +25,7 @@
 //
 // A row is divided among a cluster of 1 to 8 CTAs, as many as leave every SM with work.  The row is
 // read two or three times, the first time from memory, then from the L2 cache.  Bound: for few rows the chain of
-// cluster barriers, for many the fp64 units (12 operations per token at half a warp per clock each).
+// cluster barriers, for many the fp64 units (nine operations per token at half a clock per warp each).
 #include <math.h>
 
 #include "df11_launch.h"
@@ -36,8 +36,10 @@ constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 4096;
 constexpr int kList = 2048;
+constexpr int kFew = 128;                     // numbers that are compared with one another
 constexpr int kBlocks = kThreads;             // block sums per CTA, at most
 constexpr int kFewTokens = 256;               // top-k up to here goes by the threads' largest
+constexpr int kFewListed = 64;                // lists up to here are drawn from without sorting
 constexpr uint32_t kLowestKey = 0x00800000u;  // key of the lowest finite float
 constexpr uint32_t kAny = 0xFFFFFFFFu;
 
@@ -55,47 +57,57 @@ __device__ __forceinline__ float logit_of(uint32_t key)
     return __uint_as_float(key & 0x80000000u ? key & 0x7FFFFFFFu : ~key);
 }
 
-// Weights exp((z - c) / T) 2^S, in fp64 to 2^-48 of themselves and rounded to integers.
-// With t = 32 (z - c) / (T ln 2), n the nearest integer and f = t - n:  2^(t/32) = 2^(n/32) 2^(f/32);
-// the first factor is one of 32 numbers times a power of two, the second the Taylor sum of
-// exp(f ln2 / 32) up to the fifth power (|f ln2 / 32| < 0.011, remainder below 3e-15).
-constexpr int kRoots = 32;
+// Weights exp((z - c) / T) 2^S, in fp64 to 2^-44 of themselves and rounded to integers.
+// With t = 64 (z - c) / (T ln 2), n an integer next to it and f = t - n:  2^(t/64) = 2^(n/64) 2^(f/64);
+// the first factor is one of 64 numbers times a power of two, the second the Taylor sum of exp(f ln2 / 64)
+// up to the fourth power (|f ln2 / 64| < 0.0055, remainder below 5e-14).  n is found in fp32, which leaves nine
+// fp64 operations.
+constexpr int kRoots = 64;
 constexpr double kOne52 = 4503599627370496.0;  // 2^52: added to a number below it, the sum's low bits are the nearest integer
 struct Weigher {
     float cap, cut;                           // the largest logit that counts, and one below which a weight is less than 2^-60
-    bool plain;                               // -inf gets no weight by itself; otherwise the caller must not ask
+    float half, slope32;                      // -cap / 2; twice the slope
+    bool plain;                               // fast() may be asked for any logit, -inf included
     double peak, slope, unit;
     int shift;                                // S
-    const double *roots;                      // 2^(j/32), in shared memory
+    const double *roots;                      // 2^(j/64), in shared memory
 
     __device__ __forceinline__ Weigher(float best, double t, int s, const double *r) : shift(s), roots(r)
     {
         constexpr float kMost = 3.402823466e38f;
         cap = fminf(best, kMost);
         const float low = (float)fmax(cap - 60.0 * 0.69314718055994530942 * t, -(double)kMost);
-        plain = best <= kMost && low > -kMost;
         cut = low > -kMost ? logit_of(key_of(low) - 1) : low;     // rounded down
         peak = (double)cap;
-        // the second where even the float below the largest is thousands of octaves away
-        slope = fmin(kRoots * 1.4426950408889634074 / t, 0x1p30 / (peak - (double)cut));
+        slope = fmin(kRoots * 1.4426950408889634074 / t, 1e300);
+        slope32 = (float)fmin(2.0 * slope, 1e38);
+        half = -0.5f * cap;
+        plain = best <= kMost && low > -kMost && (peak - (double)cut) * slope < 70.0 * kRoots;
         unit = ldexp(1.0, s);
     }
-    // exactly 2^S for the largest; less than 1/2 for what is below `cut`, -inf included
-    __device__ __forceinline__ double real(float z) const
+    // For logits from `cut` to `cap`; exactly 2^S for the largest.
+    __device__ __forceinline__ double inner(float z) const
     {
-        constexpr double kMagic = 1.5 * kOne52;
         constexpr double a = 0.69314718055994530942 / kRoots;
-        const double t = ((double)fminf(fmaxf(z, cut), cap) - peak) * slope;
-        const double m = t + kMagic;
-        const int n = max(__double2loint(m), -63 * kRoots);
-        const double f = t - (m - kMagic);
-        double p = fma(a * a * a * a * a / 120, f, a * a * a * a / 24);
-        p = fma(p, f, a * a * a / 6);
+        // halves: the whole difference may not fit a float.  The sum with 1.5 * 2^23 has the integer in its low bits
+        const int n = __float_as_int(fmaf(fmaf(z, 0.5f, half), slope32, 12582912.0f)) - 0x4B400000;
+        const double k = __hiloint2double(0x43300000, n ^ 0x80000000) - (kOne52 + 2147483648.0);
+        const double f = fma((double)z - peak, slope, -k);
+        double p = fma(a * a * a * a / 24, f, a * a * a / 6);
         p = fma(p, f, a * a / 2);
         p = fma(p, f, a);
         const double root = roots[n & (kRoots - 1)];
-        const double scaled = __hiloint2double(__double2hiint(root) + (n & -kRoots) * (1 << 15) + (shift << 20), __double2loint(root));
+        const double scaled = __hiloint2double(__double2hiint(root) + (n & -kRoots) * ((1 << 20) / kRoots) + (shift << 20),
+                                               __double2loint(root));
         return fma(scaled, p * f, scaled);
+    }
+    // Where `plain`: less than 1/2 for what is below `cut`, -inf included.
+    __device__ __forceinline__ double fast(float z) const { return inner(fmaxf(z, cut)); }
+    // 0 below `cut`; whatever lies above `cap` counts as it.
+    __device__ __forceinline__ double real(float z) const
+    {
+        const double w = inner(z >= cut ? fminf(z, cap) : cap);
+        return z >= cut && (z == cap || (peak - (double)fminf(z, cap)) * slope < 70.0 * kRoots) ? w : 0.0;
     }
     // The nearest integer to w < 2^51, plus kBias; sums of such numbers are put right by as many kBias.
     static constexpr u64 kBias = 0x4330000000000000ull;
@@ -127,15 +139,20 @@ struct Verdict {         // what the first CTA finds on its list
 };
 
 struct Shared {
-    uint32_t count[kBins];                    // this CTA's counts
+    alignas(16) uint32_t count[kBins];        // this CTA's counts
     uint32_t merged[kBins];                   // the row's
     u64 list[kList], weight[kList];
     u64 blocks[kBlocks];
     u64 partial[kWarps];
-    double partial_real[kWarps], roots[kRoots];
+    double roots[kRoots];
+    float partial_real[kWarps];
+    uint32_t partial_count[kWarps];
     float partial_top[kWarps], partial_bottom[kWarps];
     Exchange mine;
     Verdict verdict;
+    u64 few[kFew], few_measure[kFew], partial_most[kWarps], border;         // find_border's
+    uint32_t parts_low[kThreads], parts_high[kThreads];
+    uint32_t few_n, part;
     uint32_t list_n, found;
     int bin_k, bin_p, bin_low, bin_high;      // interval of the top-k border; of the top-p border, and those around it
     uint32_t above_k, above_low, upto_high;   // tokens above bin_k; above bin_low; and down to bin_high
@@ -189,62 +206,89 @@ template <typename V> __device__ V block_scan(V x, V *partial, V *total)
     return before + sum - x;
 }
 
-// Sorts list[0 .. n) of different numbers in descending order (n <= kList); what is behind it, up to a
-// power of two, is lost.
-__device__ __noinline__ void sort_list(u64 *list, int n)
-{
-    if (n <= kThreads / 2) {                  // few: every number's place is how many are larger
-        u64 x = 0;
-        int place = 0;
-        if ((int)threadIdx.x < n) {
-            x = list[threadIdx.x];
-#pragma unroll 8
-            for (int i = 0; i < n; ++i) place += list[i] > x;
-        }
-        __syncthreads();
-        if ((int)threadIdx.x < n) list[place] = x;
-        __syncthreads();
-        return;
-    }
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + threadIdx.x; i < size; i += kThreads) list[i] = 0;
-    __syncthreads();
-    for (int span = 2; span <= size; span <<= 1)
-        for (int step = span >> 1; step; step >>= 1) {
-            for (int i = threadIdx.x; i < size / 2; i += kThreads) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const u64 x = list[a], y = list[b];
-                if ((x < y) == ((a & span) == 0)) list[a] = y, list[b] = x;
-            }
-            __syncthreads();
-        }
-}
-
 __device__ __forceinline__ u64 listed(float z, uint32_t index) { return (u64)key_of(z) << 32 | (0xFFFFFFFFu - index); }
 __device__ __forceinline__ float listed_logit(u64 x) { return logit_of((uint32_t)(x >> 32)); }
 __device__ __forceinline__ uint32_t listed_index(u64 x) { return 0xFFFFFFFFu - (uint32_t)x; }
 
-// Running sums of weigh(logit) over list[0 .. n), in `sums`; the whole sum is returned.
-template <typename K> __device__ u64 scan_list(const u64 *list, int n, u64 *sums, u64 *partial, K logit, const Weigher &weigh)
+// The least of the different numbers key(0) .. key(n - 1) up to which the measures sum to `want` or more
+// (1 <= want <= the sum of all).  The numbers' range is divided among the threads, the measures are added up there,
+// and the part in which the border lies is divided again, until so few are left that every number can be
+// compared with every other.
+template <typename K, typename M> __device__ __noinline__ u64 find_border(int n, K key, M measure, u64 want, Shared &s)
 {
-    constexpr int kEach = kList / kThreads;
-    u64 w[kEach], mine = 0, total;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 low = 0, high = ~0ull;
+    for (bool first = true;; first = false) {
+        // what is left, and its range
+        u64 least = ~0ull, most = 0;
+        __syncthreads();
+        if (tid == 0) s.few_n = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 x = key(i);
+            if (x < low || x > high) continue;
+            least = min(least, x), most = max(most, x);
+            if (first && n > kFew) continue;
+            const uint32_t at = atomicAdd(&s.few_n, 1u);
+            if (at < (uint32_t)kFew) s.few[at] = x, s.few_measure[at] = measure(i);
+        }
 #pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = threadIdx.x * kEach + j;
-        w[j] = i < n ? weigh(logit(list[i])) : 0;
-        mine += w[j];
+        for (int d = 16; d; d >>= 1) {
+            least = min(least, __shfl_xor_sync(0xffffffffu, least, d));
+            most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+        }
+        if (lane == 0) s.partial[warp] = least, s.partial_most[warp] = most;
+        __syncthreads();
+        const int few = (int)s.few_n;
+        if (few > 0 && few <= kFew) {
+            if (tid < few) {
+                const u64 x = s.few[tid], m = s.few_measure[tid];
+                u64 ahead = 0;
+#pragma unroll 4
+                for (int j = 0; j < few; ++j) ahead += s.few[j] < x ? s.few_measure[j] : 0;
+                if (ahead < want && want <= ahead + m) s.border = x;
+            }
+            __syncthreads();
+            return s.border;
+        }
+        low = ~0ull, high = 0;
+        for (int w = 0; w < kWarps; ++w) low = min(low, s.partial[w]), high = max(high, s.partial_most[w]);
+        const int shift = max(64 - __clzll(high - low) - 9, 0);             // 512 parts
+        s.parts_low[tid] = s.parts_high[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            const u64 x = key(i);
+            if (x < low || x > high) continue;
+            // two additions of 32 bits: one of 64 in shared memory is a loop that many equal parts would stall
+            const u64 m = measure(i);
+            const uint32_t at = (uint32_t)((x - low) >> shift), m0 = (uint32_t)m;
+            const uint32_t was = atomicAdd(&s.parts_low[at], m0), carry = (uint32_t)(was + m0) < was;
+            if ((uint32_t)(m >> 32) + carry) atomicAdd(&s.parts_high[at], (uint32_t)(m >> 32) + carry);
+        }
+        __syncthreads();
+        u64 all;
+        const u64 mine = (u64)s.parts_high[tid] << 32 | s.parts_low[tid], before = block_scan(mine, s.partial, &all);
+        if (before < want && want <= before + mine) s.part = tid, s.base = before;
+        __syncthreads();
+        want -= s.base;
+        low += (u64)s.part << shift;
+        if (shift == 0) return low;
+        high = min(high, low + ((u64)1 << shift) - 1);
     }
-    u64 run = block_scan(mine, partial, &total);
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) {
-        const int i = threadIdx.x * kEach + j;
-        run += w[j];
-        if (i < n) sums[i] = run;
-    }
+}
+
+// Weights of the logits on the list.
+__device__ __forceinline__ void weigh_list(int n, const Weigher &weigh, Shared &s)
+{
+    for (int i = threadIdx.x; i < n; i += kThreads) s.weight[i] = weigh(listed_logit(s.list[i]));
     __syncthreads();
-    return total;
+}
+
+__device__ __forceinline__ u64 list_mass(int n, Shared &s)
+{
+    u64 mass = 0;
+    for (int i = threadIdx.x; i < n; i += kThreads) mass += s.weight[i];
+    return block_sum(mass, s.partial);
 }
 
 __device__ __forceinline__ u64 share_of(double p, u64 total) { return max((u64)ceil(fmax(p, 0.0) * (double)total), 1ull); }
@@ -394,32 +438,68 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
 }
 
 // ---------------------------------------------------------------------------------------------
+// A list of at most one token per thread, in any order: every thread finds its token's rank, the mass before
+// it in that order, and the kept mass before it by index, by looking at all others.
+__device__ __forceinline__ void draw_from_few(int n, const Row &row, const Weigher &weigh, Shared &s, int64_t *out)
+{
+    const int tid = threadIdx.x;
+    const u64 me = tid < n ? s.list[tid] : 0;
+    const double real = tid < n ? weigh.real(listed_logit(me)) : 0.0;
+    const u64 w = tid < n ? weigh.biased(real) - weigh.kBias : 0;
+    if (tid < n) s.weight[tid] = w;
+    __syncthreads();
+    int rank = 0;
+    u64 before = 0;
+    const bool by_mass = row.p < 1.0;
+    if (tid < n) {
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) {
+            const bool ahead = s.list[i] > me;
+            rank += ahead;
+            if (by_mass) before += ahead ? s.weight[i] : 0;
+        }
+    }
+    bool kept = tid < n && (row.k <= 0 || rank < row.k);
+    if (by_mass) {
+        const u64 total = block_sum(kept ? w : 0, s.partial);
+        kept = kept && (rank == 0 || before < share_of(row.p, total));
+    }
+    kept = kept && real >= row.low * weigh.unit;
+    __syncthreads();
+    if (tid < n) s.weight[tid] = kept ? w : 0;
+    const u64 total = block_sum(kept ? w : 0, s.partial), want = draw_of(row.u, total);
+    if (kept) {
+        u64 upto = w;
+        const uint32_t index = (uint32_t)me;                     // larger for a lower index
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) upto += (uint32_t)s.list[i] > index ? s.weight[i] : 0;
+        if (upto > want && upto - w <= want) *out = listed_index(me);
+    }
+}
+
 // The list holds the highest-ranked n tokens of the row, at least those that top-k keeps: all filters and the draw.
 __device__ __noinline__ void draw_from_list(int n, const Row &row, const Weigher &weigh, Shared &s, int64_t *out)
 {
-    sort_list(s.list, n);
-    if (row.k > 0 && row.k < n) n = (int)row.k;
-    if (row.p < 1.0) {
-        const u64 want = share_of(row.p, scan_list(s.list, n, s.weight, s.partial, listed_logit, weigh));
-        int fit = 0;
-        for (int i = threadIdx.x; i < n; i += kThreads) fit += i == 0 || s.weight[i - 1] < want;
-        n = (int)block_sum((u64)fit, s.partial);
-    }
+    if (n <= kFewListed) return draw_from_few(n, row, weigh, s, out);
+    weigh_list(n, weigh, s);
+    auto by_rank = [&](int i) { return ~s.list[i]; };
+    auto mass = [&](int i) { return s.weight[i]; };
+    auto drop_behind = [&](u64 border) {
+        for (int i = threadIdx.x; i < n; i += kThreads)
+            if (by_rank(i) > border) s.weight[i] = 0;
+        __syncthreads();
+    };
+    if (row.k > 0 && row.k < n) drop_behind(find_border(n, by_rank, [](int) { return (u64)1; }, (u64)row.k, s));
+    if (row.p < 1.0) drop_behind(find_border(n, by_rank, mass, share_of(row.p, list_mass(n, s)), s));
     if (row.low > 0.0) {                      // min-p
-        int fit = 0;
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const float z = listed_logit(s.list[i]);
-            fit += weigh.real(z) >= row.low * weigh.unit;
-        }
-        n = (int)block_sum((u64)fit, s.partial);
+        const double floor = row.low * weigh.unit;
+        for (int i = threadIdx.x; i < n; i += kThreads)
+            if (weigh.real(listed_logit(s.list[i])) < floor) s.weight[i] = 0;
+        __syncthreads();
     }
-    for (int i = threadIdx.x; i < n; i += kThreads) s.list[i] = s.list[i] << 32 | s.list[i] >> 32;   // now by index
-    __syncthreads();
-    sort_list(s.list, n);
-    const u64 kept = scan_list(s.list, n, s.weight, s.partial, [](u64 x) { return logit_of((uint32_t)x); }, weigh);
-    const u64 want = draw_of(row.u, kept);
-    for (int i = threadIdx.x; i < n; i += kThreads)
-        if (s.weight[i] > want && (i == 0 || s.weight[i - 1] <= want)) *out = 0xFFFFFFFFu - (uint32_t)(s.list[i] >> 32);
+    const u64 want = draw_of(row.u, list_mass(n, s)) + 1;
+    const u64 index = find_border(n, [&](int i) { return (u64)listed_index(s.list[i]); }, mass, want, s);
+    if (threadIdx.x == 0) *out = (int64_t)index;
 }
 
 struct SampleArgs {
@@ -596,42 +676,50 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             s.bin_k = s.bin_p = s.bin_high = kBins - 1, s.above_k = s.bin_low = s.above_low = 0;
             s.verdict.fallback = 0;
         }
-        u64 mine = 0, whole;
-        for (int j = 0; j < kEach; ++j) mine += count[tid * kEach + j];
-        const u64 ahead = block_scan(mine, s.partial, &whole);
-        if (tid == 0) s.upto_high = (uint32_t)whole;
-        const u64 limit = by_rank ? min((u64)row.k, whole) : whole;
-        const double step = scale > 0.0f ? -fmin(1.0 / row.t, 1e300) / scale : 0.0;
-        double mass[kEach], sum = 0.0;
+        uint32_t c[kEach], mine = 0, whole;
+#pragma unroll
+        for (int j = 0; j < kEach; j += 4) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(count + tid * kEach + j);
+            c[j] = x.x, c[j + 1] = x.y, c[j + 2] = x.z, c[j + 3] = x.w;
+            mine += x.x + x.y + x.z + x.w;
+        }
+        const uint32_t ahead = block_scan(mine, s.partial_count, &whole);
+        if (tid == 0) s.upto_high = whole;
+        const uint32_t limit = by_rank ? (uint32_t)min(row.k, (long long)whole) : whole;
+        // an interval's width in octaves; its tokens weigh what its middle weighs, to half of that
+        const float width = scale > 0.0f ? (float)fmin(1.4426950408889634074 / row.t / scale, 1e30) : 0.0f;
+        float mass[kEach], sum = 0.0f, squares = 0.0f;
         {
-            u64 n = ahead;
+            uint32_t n = ahead;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const int bin = tid * kEach + j;
-                const u64 c = count[bin];
-                if (n < limit && n + c >= limit) s.bin_k = bin, s.above_k = (uint32_t)n;
-                mass[j] = by_mass && c && n < limit ? (double)min(c, limit - n) * exp(step * (bin + 0.5)) : 0.0;
+                if (n < limit && n + c[j] >= limit) s.bin_k = bin, s.above_k = n;
+                mass[j] = by_mass && c[j] && n < limit ? (float)min(c[j], limit - n) * exp2f(-width * (bin + 0.5f)) : 0.0f;
                 sum += mass[j];
-                n += c;
+                squares += mass[j] * mass[j];
+                n += c[j];
             }
         }
         if (by_mass) {
-            // an interval's mass is off by half its width at most, so the border is off by that of all masses
-            double all, run = block_scan(sum, s.partial_real, &all);
-            const double want = fmax(row.p, 0.0) * all, margin = 2.1 * expm1(-0.5 * step) * all;
-            u64 n = ahead;
+            float all, run = block_scan(sum, s.partial_real, &all);
+            // The border's place is off by what the masses before it and their sum are.  No interval is off by
+            // more than half its width, which bounds it; if they are off independently of one another,
+            // by a tenth of that or less, for which five standard deviations are allowed here.
+            const float spread = sqrtf(block_sum(squares, s.partial_real)) * (0.2f * width) * 10.0f + 1e-5f * all;
+            const float want = (float)fmax(row.p, 0.0) * all, margin = fminf(2.1f * (exp2f(0.5f * width) - 1.0f) * all + 1e-5f * all, spread);
+            uint32_t n = ahead;
 #pragma unroll
             for (int j = 0; j < kEach; ++j) {
                 const int bin = tid * kEach + j;
-                const u64 c = count[bin];
-                const double next = run + mass[j];
-                if (mass[j] > 0.0) {
+                const float next = run + mass[j];
+                if (mass[j] > 0.0f) {
                     if (run < want && next >= want) s.bin_p = bin;
-                    if (run < want - margin && next >= want - margin) s.bin_low = bin, s.above_low = (uint32_t)n;
-                    if (run < want + margin && next >= want + margin) s.bin_high = bin, s.upto_high = (uint32_t)(n + c);
+                    if (run < want - margin && next >= want - margin) s.bin_low = bin, s.above_low = n;
+                    if (run < want + margin && next >= want + margin) s.bin_high = bin, s.upto_high = n + c[j];
                 }
                 run = next;
-                n += c;
+                n += c[j];
             }
         }
         __syncthreads();
@@ -658,11 +746,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     draw_from_list((int)s.list_n, row, weigh, s, a.out + at);
                     if (tid == 0) s.verdict.fallback = 2;
                 } else {
-                    sort_list(s.list, (int)s.list_n);
-                    if (tid == 0) {
-                        const u64 last = s.list[limit - s.above_k - 1];
-                        s.verdict.logit = listed_logit(last), s.verdict.index = listed_index(last);
-                    }
+                    const u64 last = ~find_border((int)s.list_n, [&](int i) { return ~s.list[i]; }, [](int) { return (u64)1; },
+                                                  (u64)(limit - s.above_k), s);
+                    if (tid == 0) s.verdict.logit = listed_logit(last), s.verdict.index = listed_index(last);
                 }
                 __syncthreads();
                 if (tid == 0) s.list_n = 0;
@@ -705,7 +791,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                         for (int j = 0; j < 8; ++j) {
                             const bool kept = !ranked.value || is_kept(z[j], index + j);
                             const float place = place_of(ranked.value ? fminf(z[j], from) : z[j]);
-                            const double w = weigh.real(z[j]);
+                            const double w = ranked.value ? weigh.real(z[j]) : weigh.fast(z[j]);
                             const u64 all = weigh.biased(kept ? w : 0.0);
                             mass_all += all;
                             above += place < low ? all : weigh.kBias;
@@ -740,20 +826,19 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 }
                 const u64 want = share_of(row.p, mass_all);
                 const int n = (int)min(s.list_n, (uint32_t)kList);
-                sort_list(s.list, n);
-                const u64 on_list = scan_list(s.list, n, s.weight, s.partial, listed_logit, weigh);
+                weigh_list(n, weigh, s);
+                const u64 on_list = list_mass(n, s);
                 if (s.list_n > (uint32_t)kList || mass_above >= want || mass_above + on_list < want) {
                     if (tid == 0) s.verdict.fallback = 1;
                 } else {
+                    const u64 last = find_border(n, [&](int i) { return ~s.list[i]; }, [&](int i) { return s.weight[i]; },
+                                                 want - mass_above, s);
+                    if (tid == 0) s.verdict.logit = listed_logit(~last), s.verdict.index = listed_index(~last);
                     for (int i = tid; i < n; i += kThreads) {
-                        const u64 before = mass_above + (i ? s.weight[i - 1] : 0), after = mass_above + s.weight[i];
-                        if (before >= want) continue;
-                        const float z = listed_logit(s.list[i]);
+                        if (~s.list[i] > last || (floor > 0.0 && weigh.real(listed_logit(s.list[i])) < floor)) continue;
                         const uint32_t index = listed_index(s.list[i]);
-                        if (after >= want) s.verdict.logit = z, s.verdict.index = index;
-                        if (weigh.real(z) < floor) continue;
                         const uint32_t block = (index + tokens.lead) / 8 / block_groups, owner = block / my_blocks;
-                        atomicAdd(&(size > 1 ? remote(&s, owner) : &s)->blocks[block - owner * my_blocks], after - before);
+                        atomicAdd(&(size > 1 ? remote(&s, owner) : &s)->blocks[block - owner * my_blocks], s.weight[i]);
                     }
                 }
             }
@@ -778,7 +863,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     tokens.logits(g, z);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const double w = weigh.real(z[j]);
+                        const double w = filtered.value ? weigh.real(z[j]) : weigh.fast(z[j]);
                         part += weigh.biased(!filtered.value || (is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor) ? w : 0.0);
                     }
                     part -= 8 * weigh.kBias;
