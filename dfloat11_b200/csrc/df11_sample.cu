@@ -39,7 +39,6 @@ constexpr int kList = 2048;
 constexpr int kFew = 128;                     // numbers that are compared with one another
 constexpr int kBlocks = kThreads;             // block sums per CTA, at most
 constexpr int kFewTokens = 256;               // top-k up to here goes by the threads' largest
-constexpr int kFewListed = 64;                // lists up to here are drawn from without sorting
 constexpr uint32_t kLowestKey = 0x00800000u;  // key of the lowest finite float
 constexpr uint32_t kAny = 0xFFFFFFFFu;
 
@@ -159,6 +158,11 @@ struct Shared {
     u64 base;
 };
 
+// The block's shared memory.  Functions that are not inlined name it themselves: through a reference handed to
+// them every access would have to find out first which memory it goes to.
+extern __shared__ __align__(16) unsigned char raw_shared[];
+#define DF11_SHARED Shared &s = *reinterpret_cast<Shared *>(raw_shared)
+
 __device__ __forceinline__ void cluster_sync(uint32_t size)
 {
     if (size > 1) asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
@@ -214,8 +218,9 @@ __device__ __forceinline__ uint32_t listed_index(u64 x) { return 0xFFFFFFFFu - (
 // (1 <= want <= the sum of all).  The numbers' range is divided among the threads, the measures are added up there,
 // and the part in which the border lies is divided again, until so few are left that every number can be
 // compared with every other.
-template <typename K, typename M> __device__ __noinline__ u64 find_border(int n, K key, M measure, u64 want, Shared &s)
+template <typename K, typename M> __device__ __noinline__ u64 find_border(int n, K key, M measure, u64 want)
 {
+    DF11_SHARED;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     u64 low = 0, high = ~0ull;
     for (bool first = true;; first = false) {
@@ -241,13 +246,19 @@ template <typename K, typename M> __device__ __noinline__ u64 find_border(int n,
         __syncthreads();
         const int few = (int)s.few_n;
         if (few > 0 && few <= kFew) {
-            if (tid < few) {
-                const u64 x = s.few[tid], m = s.few_measure[tid];
-                u64 ahead = 0;
+            // kThreads / kFew threads per number, each compares it with as large a part of the others
+            constexpr int kWays = kThreads / kFew;
+            const int mine = tid / kWays;
+            const u64 x = mine < few ? s.few[mine] : 0, m = mine < few ? s.few_measure[mine] : 0;
+            u64 ahead = 0;
 #pragma unroll 4
-                for (int j = 0; j < few; ++j) ahead += s.few[j] < x ? s.few_measure[j] : 0;
-                if (ahead < want && want <= ahead + m) s.border = x;
+            for (int j = tid % kWays; j < few; j += kWays) {
+                const u64 y = s.few[j], z = s.few_measure[j];
+                ahead += y < x ? z : 0;
             }
+#pragma unroll
+            for (int d = kWays / 2; d; d >>= 1) ahead += __shfl_xor_sync(0xffffffffu, ahead, d);
+            if (mine < few && ahead < want && want <= ahead + m) s.border = x;
             __syncthreads();
             return s.border;
         }
@@ -277,15 +288,31 @@ template <typename K, typename M> __device__ __noinline__ u64 find_border(int n,
     }
 }
 
+// Orders and measures of the tokens on the list.
+struct ByRank {
+    __device__ __forceinline__ u64 operator()(int i) const { DF11_SHARED; return ~s.list[i]; }
+};
+struct ByIndex {
+    __device__ __forceinline__ u64 operator()(int i) const { DF11_SHARED; return listed_index(s.list[i]); }
+};
+struct ByCount {
+    __device__ __forceinline__ u64 operator()(int) const { return 1; }
+};
+struct ByMass {
+    __device__ __forceinline__ u64 operator()(int i) const { DF11_SHARED; return s.weight[i]; }
+};
+
 // Weights of the logits on the list.
-__device__ __forceinline__ void weigh_list(int n, const Weigher &weigh, Shared &s)
+__device__ __forceinline__ void weigh_list(int n, const Weigher &weigh)
 {
+    DF11_SHARED;
     for (int i = threadIdx.x; i < n; i += kThreads) s.weight[i] = weigh(listed_logit(s.list[i]));
     __syncthreads();
 }
 
-__device__ __forceinline__ u64 list_mass(int n, Shared &s)
+__device__ __forceinline__ u64 list_mass(int n)
 {
+    DF11_SHARED;
     u64 mass = 0;
     for (int i = threadIdx.x; i < n; i += kThreads) mass += s.weight[i];
     return block_sum(mass, s.partial);
@@ -337,8 +364,9 @@ template <typename T> struct Tokens {
 // The key in which the running measure (from the largest key down) reaches `want`, and the measure
 // above it.
 template <typename T, typename M>
-__device__ void descend(const Tokens<T> &tokens, float lowest, u64 want, M measure, Shared &s, float *found, u64 *above)
+__device__ void descend(const Tokens<T> &tokens, float lowest, u64 want, M measure, float *found, u64 *above)
 {
+    DF11_SHARED;
     u64 *digits = s.list;
     uint32_t prefix = 0;
     u64 over = 0;
@@ -369,8 +397,9 @@ __device__ void descend(const Tokens<T> &tokens, float lowest, u64 want, M measu
     *above = over;
 }
 
-template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T> &tokens, const Row &row, float lowest, const Weigher &weigh, Shared &s, int64_t *out)
+template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T> &tokens, const Row &row, float lowest, const Weigher &weigh, int64_t *out)
 {
+    DF11_SHARED;
     const int tid = threadIdx.x;
     const uint32_t vocab = tokens.vocab;
     float kept = lowest;
@@ -380,7 +409,7 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
         for (uint32_t i = tid; i < vocab; i += kThreads) alive += tokens.at(i) >= lowest;
         alive = block_sum(alive, s.partial);
         if ((u64)row.k < alive) {
-            descend(tokens, lowest, (u64)row.k, [](float) { return (u64)1; }, s, &kept, &above);
+            descend(tokens, lowest, (u64)row.k, [](float) { return (u64)1; }, &kept, &above);
             ties_kept = (u64)row.k - above;
         }
     }
@@ -399,7 +428,7 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
         if (want <= mass) {                       // the border lies above the ties of top-k
             float z;
             const float before = kept;
-            descend(tokens, lowest, want, [&](float x) { return x > before ? weigh(x) : (u64)0; }, s, &z, &above);
+            descend(tokens, lowest, want, [&](float x) { return x > before ? weigh(x) : (u64)0; }, &z, &above);
             const u64 w = weigh(z);
             kept = z;
             ties_kept = (want - above + w - 1) / w;
@@ -438,67 +467,92 @@ template <typename T> __device__ __noinline__ void sample_slowly(const Tokens<T>
 }
 
 // ---------------------------------------------------------------------------------------------
-// A list of at most one token per thread, in any order: every thread finds its token's rank, the mass before
-// it in that order, and the kept mass before it by index, by looking at all others.
-__device__ __forceinline__ void draw_from_few(int n, const Row &row, const Weigher &weigh, Shared &s, int64_t *out)
+// A short list, in any order: every token's rank, the mass before it in that order, and the kept mass
+// before it by index come from comparing it with all others, by WAYS threads per token.
+template <int WAYS> __device__ __forceinline__ void draw_from_few(int n, const Row &row, const Weigher &weigh, int64_t *out)
 {
-    const int tid = threadIdx.x;
-    const u64 me = tid < n ? s.list[tid] : 0;
-    const double real = tid < n ? weigh.real(listed_logit(me)) : 0.0;
-    const u64 w = tid < n ? weigh.biased(real) - weigh.kBias : 0;
-    if (tid < n) s.weight[tid] = w;
+    DF11_SHARED;
+    const int tid = threadIdx.x, mine = tid / WAYS, way = tid % WAYS;
+    const bool some = mine < n;
+    const u64 me = some ? s.list[mine] : 0;
+    const double real = some ? weigh.real(listed_logit(me)) : 0.0;
+    const u64 w = weigh.biased(real) - weigh.kBias;
+    if (some && way == 0) s.weight[mine] = w;
     __syncthreads();
     int rank = 0;
     u64 before = 0;
-    const bool by_mass = row.p < 1.0;
-    if (tid < n) {
 #pragma unroll 4
-        for (int i = 0; i < n; ++i) {
-            const bool ahead = s.list[i] > me;
-            rank += ahead;
-            if (by_mass) before += ahead ? s.weight[i] : 0;
-        }
+    for (int i = way; i < n; i += WAYS) {
+        const u64 x = s.list[i], y = s.weight[i];
+        rank += x > me;
+        before += x > me ? y : 0;
     }
-    bool kept = tid < n && (row.k <= 0 || rank < row.k);
-    if (by_mass) {
-        const u64 total = block_sum(kept ? w : 0, s.partial);
+#pragma unroll
+    for (int d = WAYS / 2; d; d >>= 1) {
+        rank += __shfl_xor_sync(0xffffffffu, rank, d);
+        before += __shfl_xor_sync(0xffffffffu, before, d);
+    }
+    bool kept = some && (row.k <= 0 || rank < row.k);
+    if (row.p < 1.0) {
+        const u64 total = block_sum(kept && way == 0 ? w : 0, s.partial);
         kept = kept && (rank == 0 || before < share_of(row.p, total));
     }
     kept = kept && real >= row.low * weigh.unit;
     __syncthreads();
-    if (tid < n) s.weight[tid] = kept ? w : 0;
-    const u64 total = block_sum(kept ? w : 0, s.partial), want = draw_of(row.u, total);
-    if (kept) {
-        u64 upto = w;
-        const uint32_t index = (uint32_t)me;                     // larger for a lower index
+    if (some && way == 0) s.weight[mine] = kept ? w : 0;
+    const u64 total = block_sum(kept && way == 0 ? w : 0, s.partial), want = draw_of(row.u, total);
+    u64 upto = 0;
+    const uint32_t index = (uint32_t)me;                         // larger for a lower index
 #pragma unroll 4
-        for (int i = 0; i < n; ++i) upto += (uint32_t)s.list[i] > index ? s.weight[i] : 0;
-        if (upto > want && upto - w <= want) *out = listed_index(me);
+    for (int i = way; i < n; i += WAYS) {
+        const uint32_t x = (uint32_t)s.list[i];
+        const u64 y = s.weight[i];
+        upto += x > index ? y : 0;
     }
+#pragma unroll
+    for (int d = WAYS / 2; d; d >>= 1) upto += __shfl_xor_sync(0xffffffffu, upto, d);
+    if (kept && upto <= want && want < upto + w) *out = listed_index(me);
 }
 
 // The list holds the highest-ranked n tokens of the row, at least those that top-k keeps: all filters and the draw.
-__device__ __noinline__ void draw_from_list(int n, const Row &row, const Weigher &weigh, Shared &s, int64_t *out)
+__device__ __noinline__ void draw_from_list(int n, const Row &row, const Weigher &weigh, int64_t *out)
 {
-    if (n <= kFewListed) return draw_from_few(n, row, weigh, s, out);
-    weigh_list(n, weigh, s);
-    auto by_rank = [&](int i) { return ~s.list[i]; };
-    auto mass = [&](int i) { return s.weight[i]; };
+    DF11_SHARED;
+    if (n > kFew && row.k > 0 && row.k <= kFew) {
+        // only what top-k keeps stays on the list
+        const u64 border = find_border(n, ByRank(), ByCount(), (u64)row.k);
+        u64 mine[kList / kThreads];
+#pragma unroll
+        for (int j = 0; j < kList / kThreads; ++j) mine[j] = threadIdx.x + j * kThreads < n ? s.list[threadIdx.x + j * kThreads] : 0;
+        __syncthreads();
+        if (threadIdx.x == 0) s.few_n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kList / kThreads; ++j)
+            if (mine[j] && ~mine[j] <= border) s.list[atomicAdd(&s.few_n, 1u)] = mine[j];
+        __syncthreads();
+        n = (int)s.few_n;
+    }
+    if (n <= kThreads / 16) return draw_from_few<16>(n, row, weigh, out);
+    if (n <= kFew) return draw_from_few<kThreads / kFew>(n, row, weigh, out);
+    weigh_list(n, weigh);
+    const ByRank by_rank;
+    const ByMass mass;
     auto drop_behind = [&](u64 border) {
         for (int i = threadIdx.x; i < n; i += kThreads)
             if (by_rank(i) > border) s.weight[i] = 0;
         __syncthreads();
     };
-    if (row.k > 0 && row.k < n) drop_behind(find_border(n, by_rank, [](int) { return (u64)1; }, (u64)row.k, s));
-    if (row.p < 1.0) drop_behind(find_border(n, by_rank, mass, share_of(row.p, list_mass(n, s)), s));
+    if (row.k > 0 && row.k < n) drop_behind(find_border(n, by_rank, ByCount(), (u64)row.k));
+    if (row.p < 1.0) drop_behind(find_border(n, by_rank, mass, share_of(row.p, list_mass(n))));
     if (row.low > 0.0) {                      // min-p
         const double floor = row.low * weigh.unit;
         for (int i = threadIdx.x; i < n; i += kThreads)
             if (weigh.real(listed_logit(s.list[i])) < floor) s.weight[i] = 0;
         __syncthreads();
     }
-    const u64 want = draw_of(row.u, list_mass(n, s)) + 1;
-    const u64 index = find_border(n, [&](int i) { return (u64)listed_index(s.list[i]); }, mass, want, s);
+    const u64 want = draw_of(row.u, list_mass(n)) + 1;
+    const u64 index = find_border(n, ByIndex(), mass, want);
     if (threadIdx.x == 0) *out = (int64_t)index;
 }
 
@@ -516,8 +570,7 @@ struct SampleArgs {
 
 template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kernel(SampleArgs a)
 {
-    extern __shared__ __align__(16) unsigned char raw_shared[];
-    Shared &s = *reinterpret_cast<Shared *>(raw_shared);
+    DF11_SHARED;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t size = a.cluster, at = blockIdx.x / size, rank = blockIdx.x % size;
     Row row;
@@ -581,10 +634,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     }
     cluster_sync(size);
     float best = -INFINITY, least = INFINITY, bound = -INFINITY;
-    for (uint32_t r = 0; r < size; ++r) {
-        const Exchange *x = size > 1 ? remote(&s.mine, r) : &s.mine;
-        best = fmaxf(best, x->best), least = fminf(least, x->least), bound = fmaxf(bound, x->bound);
+    if (lane < (int)size) {
+        const Exchange *x = size > 1 ? remote(&s.mine, lane) : &s.mine;
+        best = x->best, least = x->least, bound = x->bound;
     }
+#pragma unroll
+    for (int d = 4; d; d >>= 1) {
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, d));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+        bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, d));
+    }
+    best = __shfl_sync(0xffffffffu, best, 0), least = __shfl_sync(0xffffffffu, least, 0), bound = __shfl_sync(0xffffffffu, bound, 0);
     if (best == -INFINITY) {                                 // nothing to draw from
         if (rank == 0 && tid == 0) {
             a.out[at] = 0;
@@ -616,8 +676,27 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     const double floor = row.low * weigh.unit;                          // weights below it are min-p's
 
     auto list_token = [&](float z, uint32_t index) {
-        const uint32_t n = atomicAdd(&head.list_n, 1u);
-        if (n < (uint32_t)kList) head.list[n] = listed(z, index);
+        const uint32_t n = atomicAdd(&s.list_n, 1u);
+        if (n < (uint32_t)kList) s.list[n] = listed(z, index);
+    };
+    // The first CTA, after a barrier: everyone's list behind its own; more than kList if they do not fit.
+    auto collect = [&]() {
+        if (size == 1) return s.list_n;
+        // every lane below the cluster's size learns one CTA's count; a warp copies one CTA's list
+        uint32_t n = lane < (int)size ? remote(&s, lane)->list_n : 0, behind = n;
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, behind, d);
+            if (lane >= d) behind += x;
+        }
+        const uint32_t all = __shfl_sync(0xffffffffu, behind, size - 1);
+        const uint32_t r = warp % size, more = __shfl_sync(0xffffffffu, n, r), at_list = __shfl_sync(0xffffffffu, behind, r) - more;
+        if (r > 0 && all <= (uint32_t)kList) {
+            const Shared &there = *remote(&s, r);
+            for (uint32_t i = warp / size * 32 + lane; i < more; i += kWarps / size * 32) s.list[at_list + i] = there.list[i];
+        }
+        __syncthreads();
+        return all;
     };
     if (few) {
         bound = fmaxf(bound, lowest);
@@ -630,9 +709,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 if (z[j] >= bound) list_token(z[j], g * 8 - tokens.lead + j);
         }
         cluster_sync(size);
+        const uint32_t n = rank == 0 ? collect() : 0;
+        if (size > 1) cluster_sync(size);
         if (rank != 0) return;
-        if (s.list_n <= (uint32_t)kList) draw_from_list((int)s.list_n, row, weigh, s, a.out + at);
-        else sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
+        if (n <= (uint32_t)kList) draw_from_list((int)n, row, weigh, a.out + at);
+        else sample_slowly(tokens, row, lowest, weigh, a.out + at);
         return;
     }
 
@@ -740,24 +821,24 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             }
             cluster_sync(size);
             if (rank == 0) {
-                if (s.list_n > (uint32_t)kList) {
+                const uint32_t n = collect();
+                if (n > (uint32_t)kList) {
                     if (tid == 0) s.verdict.fallback = 1;
                 } else if (all) {
-                    draw_from_list((int)s.list_n, row, weigh, s, a.out + at);
+                    draw_from_list((int)n, row, weigh, a.out + at);
                     if (tid == 0) s.verdict.fallback = 2;
                 } else {
-                    const u64 last = ~find_border((int)s.list_n, [&](int i) { return ~s.list[i]; }, [](int) { return (u64)1; },
-                                                  (u64)(limit - s.above_k), s);
+                    const u64 last = ~find_border((int)n, ByRank(), ByCount(),
+                                                  (u64)(limit - s.above_k));
                     if (tid == 0) s.verdict.logit = listed_logit(last), s.verdict.index = listed_index(last);
                 }
-                __syncthreads();
-                if (tid == 0) s.list_n = 0;
             }
             cluster_sync(size);
+            if (tid == 0) s.list_n = 0;
             const Verdict v = head.verdict;
             if (v.fallback) {
                 cluster_sync(size);
-                if (v.fallback == 1 && rank == 0) sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
+                if (v.fallback == 1 && rank == 0) sample_slowly(tokens, row, lowest, weigh, a.out + at);
                 return;
             }
             kept_logit = v.logit, kept_index = v.index;
@@ -777,7 +858,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             // one pass: mass of what top-k keeps, mass above the intervals, sums of blocks of the latter
             const float low = kMagic + s.bin_low, high = kMagic + s.bin_high;
             u64 mass_all = 0, mass_above = 0;
-            auto add_up = [&](auto ranked, auto floored) {
+            auto add_up = [&](auto filtered, auto plain) {
                 for (uint32_t block = warp; block < blocks; block += kWarps) {
                     u64 part = 0;
                     for (int x = 0; x < 1 << wide; ++x) {
@@ -789,18 +870,18 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                         u64 above = 0;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const bool kept = !ranked.value || is_kept(z[j], index + j);
-                            const float place = place_of(ranked.value ? fminf(z[j], from) : z[j]);
-                            const double w = ranked.value ? weigh.real(z[j]) : weigh.fast(z[j]);
+                            const bool kept = !filtered.value || is_kept(z[j], index + j);
+                            const float place = place_of(plain.value ? z[j] : fminf(z[j], from));
+                            const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
                             const u64 all = weigh.biased(kept ? w : 0.0);
                             mass_all += all;
                             above += place < low ? all : weigh.kBias;
-                            if (floored.value) part += place < low && w >= floor ? all : weigh.kBias;
+                            if (filtered.value) part += place < low && w >= floor ? all : weigh.kBias;
                             if (place >= low && place <= high && kept && z[j] >= lowest) on_list |= 1u << j;
                         }
                         mass_all -= 8 * weigh.kBias, above -= 8 * weigh.kBias;
                         mass_above += above;
-                        part += floored.value ? 0 - 8 * weigh.kBias : above;
+                        part += filtered.value ? 0 - 8 * weigh.kBias : above;
                         if (on_list) {
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
@@ -812,8 +893,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     if (lane == 0) s.blocks[block] = part;
                 }
             };
-            if (!by_rank && weigh.plain) floor > 0.0 ? add_up(No{}, Yes{}) : add_up(No{}, No{});
-            else floor > 0.0 ? add_up(Yes{}, Yes{}) : add_up(Yes{}, No{});
+            if (!weigh.plain) add_up(Yes{}, No{});
+            else if (by_rank || floor > 0.0) add_up(Yes{}, Yes{});
+            else add_up(No{}, Yes{});
             mass_all = block_sum(mass_all, s.partial);
             mass_above = block_sum(mass_above, s.partial);
             if (tid == 0) s.mine.mass = mass_all, s.mine.above = mass_above;
@@ -825,14 +907,15 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     mass_all += x->mass, mass_above += x->above;
                 }
                 const u64 want = share_of(row.p, mass_all);
-                const int n = (int)min(s.list_n, (uint32_t)kList);
-                weigh_list(n, weigh, s);
-                const u64 on_list = list_mass(n, s);
-                if (s.list_n > (uint32_t)kList || mass_above >= want || mass_above + on_list < want) {
+                const uint32_t in_all = collect();
+                const int n = (int)min(in_all, (uint32_t)kList);
+                weigh_list(n, weigh);
+                const u64 on_list = list_mass(n);
+                if (in_all > (uint32_t)kList || mass_above >= want || mass_above + on_list < want) {
                     if (tid == 0) s.verdict.fallback = 1;
                 } else {
-                    const u64 last = find_border(n, [&](int i) { return ~s.list[i]; }, [&](int i) { return s.weight[i]; },
-                                                 want - mass_above, s);
+                    const u64 last = find_border(n, ByRank(), ByMass(),
+                                                 want - mass_above);
                     if (tid == 0) s.verdict.logit = listed_logit(~last), s.verdict.index = listed_index(~last);
                     for (int i = tid; i < n; i += kThreads) {
                         if (~s.list[i] > last || (floor > 0.0 && weigh.real(listed_logit(s.list[i])) < floor)) continue;
@@ -846,14 +929,14 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             const Verdict v = head.verdict;
             if (v.fallback) {
                 cluster_sync(size);
-                if (rank == 0) sample_slowly(tokens, row, lowest, weigh, s, a.out + at);
+                if (rank == 0) sample_slowly(tokens, row, lowest, weigh, a.out + at);
                 return;
             }
             kept_logit = v.logit, kept_index = v.index;
         }
     }
     if (!by_mass) {
-        auto add_up = [&](auto filtered) {
+        auto add_up = [&](auto filtered, auto plain) {
             for (uint32_t block = warp; block < blocks; block += kWarps) {
                 u64 part = 0;
                 for (int x = 0; x < 1 << wide; ++x) {
@@ -863,7 +946,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     tokens.logits(g, z);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const double w = filtered.value ? weigh.real(z[j]) : weigh.fast(z[j]);
+                        const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
                         part += weigh.biased(!filtered.value || (is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor) ? w : 0.0);
                     }
                     part -= 8 * weigh.kBias;
@@ -873,8 +956,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                 if (lane == 0) s.blocks[block] = part;
             }
         };
-        if (by_rank || floor > 0.0 || !weigh.plain) add_up(Yes{});
-        else add_up(No{});
+        if (!weigh.plain) add_up(Yes{}, No{});
+        else if (by_rank || floor > 0.0) add_up(Yes{}, Yes{});
+        else add_up(No{}, Yes{});
     }
     // the draw: the CTA, the block, the token
     __syncthreads();
