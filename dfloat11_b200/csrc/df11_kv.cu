@@ -332,7 +332,8 @@ struct AttentionArgs {
     const int64_t *lengths, *first;
     int length_per, first_per;
     void *out;
-    float *workspace;                   // shared out: two results of rows * (D + 2) numbers per CTA
+    uint32_t *cuts;                     // shared out: per unit, the first result and the last CTA
+    float *workspace;                   // and two results of rows * (D + 2) numbers per CTA
     uint32_t batch, kv_heads, group, queries, row_groups, cluster;
     int dim, window, q_aligned;
     int64_t max_slots;
@@ -358,11 +359,16 @@ struct Sequence {
     uint32_t index, tiles, before;      // before: tiles per head of the sequences ahead of it
 };
 
+__device__ __forceinline__ int64_t length_of(const AttentionArgs &a, uint32_t b) { return clamped_length(a.lengths[a.length_per ? b : 0]); }
+__device__ __forceinline__ int64_t start_of(const AttentionArgs &a, uint32_t b)
+{
+    return a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
+}
+
 __device__ __forceinline__ uint32_t tiles_of(const AttentionArgs &a, uint32_t b)
 {
     if (b >= a.batch) return 0;
-    const int64_t length = clamped_length(a.lengths[a.length_per ? b : 0]);
-    const int64_t start = a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
+    const int64_t length = length_of(a, b), start = start_of(a, b);
     const int64_t n = sight_of(a, length, start, a.queries - 1).high - sight_of(a, length, start, 0).low + 1;
     return n > 0 ? (uint32_t)((n + 15) / 16) : 0;
 }
@@ -375,8 +381,8 @@ __device__ __forceinline__ uint32_t all_tiles(const AttentionArgs &a)
     return sum;
 }
 
-// The whole warp: the sequence that holds tile `at` (of all heads' tiles), or, by index, sequence `want`.
-template <bool BY_INDEX> __device__ __forceinline__ Sequence find_sequence(const AttentionArgs &a, uint32_t want)
+// The whole warp: the sequence that holds tile `want` of all heads' tiles.
+__device__ __forceinline__ Sequence find_sequence(const AttentionArgs &a, uint32_t want)
 {
     const uint32_t lane = threadIdx.x & 31, heads = a.kv_heads * a.row_groups;
     uint32_t before = 0;
@@ -388,7 +394,7 @@ template <bool BY_INDEX> __device__ __forceinline__ Sequence find_sequence(const
             const uint32_t x = __shfl_up_sync(0xffffffffu, sum, d);
             if (lane >= (uint32_t)d) sum += x;
         }
-        const uint32_t hit = __ballot_sync(0xffffffffu, BY_INDEX ? b0 + lane == want : (before + sum) * heads > want);
+        const uint32_t hit = __ballot_sync(0xffffffffu, (before + sum) * heads > want);
         if (hit) {
             const int at = __ffs(hit) - 1;
             return {b0 + at, __shfl_sync(0xffffffffu, mine, at), before + __shfl_sync(0xffffffffu, sum - mine, at)};
@@ -398,7 +404,13 @@ template <bool BY_INDEX> __device__ __forceinline__ Sequence find_sequence(const
     return {a.batch, 0, before};
 }
 
-__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t ctas) { return max((total + ctas - 1) / ctas, 8u); }
+// Tiles per CTA: equal parts, but no fewer than a tile per warp where the sequences have as many.
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t units, uint32_t ctas)
+{
+    return max((total + ctas - 1) / ctas, min(max(total / units, 1u), (uint32_t)kAttWarps));
+}
+
+constexpr uint32_t kNotCut = 0xFFFFFFFFu;
 
 __device__ __forceinline__ uint32_t cluster_rank()
 {
@@ -447,7 +459,8 @@ template <typename T> __device__ __forceinline__ void store4(T *p, float4 x)
 // SHARED: tiles [first_tile, last_tile) of the sequence, the result to `ws` if they are not all of them;
 // otherwise the CTAs of a cluster take equal parts.
 template <int D, int NT, int FMT, bool EXACT, bool SHARED, typename T>
-__device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, uint32_t first_tile, uint32_t last_tile, float *ws)
+__device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, int64_t length, int64_t start, uint32_t first_tile,
+                                       uint32_t last_tile, float *ws)
 {
     constexpr int kRows = NT * 8;
     constexpr int kKeyChunks = D / 64;                      // 16-byte chunks of a key row per thread
@@ -467,7 +480,71 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
     const uint32_t head = unit / a.row_groups, b = head / a.kv_heads, h = head % a.kv_heads;
     const uint32_t row0 = unit % a.row_groups * kRows, rows = a.group * a.queries, last_row = min(row0 + kRows, rows) - 1;
 
-    // the query fragments, in the order in which the key bytes lie
+    // the slots that any of the rows sees, and those that all of them see
+    const Sight top = sight_of(a, length, start, row0 / a.group), bottom = sight_of(a, length, start, last_row / a.group);
+    const int64_t low = SHARED ? sight_of(a, length, start, 0).low : top.low;
+    const int64_t n = max((SHARED ? sight_of(a, length, start, a.queries - 1).high : bottom.high) - low + 1, (int64_t)0);
+    const int inner_low = (int)min(bottom.low - low, n), inner_high = (int)max(top.high - low, (int64_t)-1);
+    const int count = (int)n;
+    int col_low[NT][2], col_high[NT][2];                    // relative to `low`
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const Sight s = sight_of(a, length, start, min(row0 + nt * 8 + 2 * c + i, last_row) / a.group);
+            col_low[nt][i] = (int)min(s.low - low, n);
+            col_high[nt][i] = (int)max(s.high - low, (int64_t)-1);
+        }
+
+    const uint32_t rank = !SHARED && a.cluster > 1 ? cluster_rank() : 0;
+    if (!SHARED) {
+        const uint32_t tiles = (uint32_t)((n + 15) / 16), share = tiles / a.cluster, extra = tiles - share * a.cluster;
+        first_tile = share * rank + min(rank, extra), last_tile = first_tile + share + (rank < extra);
+    }
+    const int begin = (int)first_tile, end = min((int)last_tile, (int)((n + 15) / 16));
+    const int64_t cell0 = (int64_t)head * a.max_slots + low;
+
+    float o[kBlocks][NT][4] = {}, o128[NT][4] = {};         // o128: 128 times the sum of the weights, in the codes' unit
+    // running maximum, sum, factor on weight * scale, and the largest weight * scale when it was set;
+    // the factor starts so large that the first weight * scale that is not zero sets it
+    float m[NT][2], l[NT][2] = {}, f[NT][2], big[NT][2] = {};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, f[nt][0] = f[nt][1] = 0x1p126f;
+
+    const int dim = EXACT ? D : a.dim;
+    // A warp's tiles come through a ring in shared memory, each operand of a tile in D / 32 copies of 512
+    // consecutive bytes.  Past the last slot the last one is copied again, and past the last chunk of a
+    // row that one: whatever lies in the cache there (a NaN, say) does not reach a product.
+    constexpr int kRowChunks = D / 16, kRowsPerCopy = 32 / kRowChunks, kCopies = 16 / kRowsPerCopy;
+    const int copy_row = lane / kRowChunks, copy_chunk_at = EXACT ? lane % kRowChunks * 16 : min(lane % kRowChunks * 16, dim - 16);
+    const uint8_t *const key_base = a.k_codes + cell0 * dim + copy_chunk_at, *const value_base = a.v_codes + cell0 * dim + copy_chunk_at;
+    uint8_t *const ring = reinterpret_cast<uint8_t *>(shared) + warp * (kStages * kStageBytes);
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    const float *const scale_base = (c < 2 ? a.k_scales : a.v_scales) + cell0;      // scales of rows r and r + 8, for all lanes of r
+    auto fetch = [&](int tile, uint32_t stage) {
+        const int s0 = tile * 16, left = count - 1 - s0;
+        const uint8_t *const kp = key_base + (int64_t)s0 * dim, *const vp = value_base + (int64_t)s0 * dim;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stage + 32 * D + lane * 4),
+                     "l"(scale_base + s0 + min(r + 8 * (c & 1), left))
+                     : "memory");
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+            const int row = i * kRowsPerCopy + copy_row, from = (left >= 15 ? row : min(row, left)) * dim;
+            const uint32_t to = stage + chunk_place<D>(row, lane % kRowChunks);
+            copy_chunk(to, kp + from);
+            copy_chunk(to + 16 * D, vp + from);
+        }
+    };
+    // which warp takes the first tile differs from CTA to CTA, so that no scheduler gets all the odd ones
+    const int turn_of = (warp + (int)blockIdx.x) & (kAttWarps - 1);
+    int ahead = begin + turn_of;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (ahead < end) fetch(ahead, ring_at + i * kStageBytes);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        ahead += kAttWarps;
+    }
+    // The query fragments, in the order in which the key bytes lie, while the first tiles are on their way.
     uint32_t qf[NT][D / 16][2];
     float mult[NT][2];                                      // score = sum * mult * key scale, in powers of two
     float offset[NT][2] = {};                               // what the sum starts from: - 128 sum(q) in the codes' unit
@@ -532,72 +609,6 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, ui
         mult[nt][1] = __shfl_sync(0xffffffffu, up, 8 * c + 4);
     }
 
-    // the slots that any of the rows sees, and those that all of them see
-    const int64_t length = clamped_length(a.lengths[a.length_per ? b : 0]);
-    const int64_t start = a.first ? clamped_length(a.first[a.first_per ? b : 0]) : 0;
-    const Sight top = sight_of(a, length, start, row0 / a.group), bottom = sight_of(a, length, start, last_row / a.group);
-    const int64_t low = SHARED ? sight_of(a, length, start, 0).low : top.low;
-    const int64_t n = max((SHARED ? sight_of(a, length, start, a.queries - 1).high : bottom.high) - low + 1, (int64_t)0);
-    const int inner_low = (int)min(bottom.low - low, n), inner_high = (int)max(top.high - low, (int64_t)-1);
-    const int count = (int)n;
-    int col_low[NT][2], col_high[NT][2];                    // relative to `low`
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const Sight s = sight_of(a, length, start, min(row0 + nt * 8 + 2 * c + i, last_row) / a.group);
-            col_low[nt][i] = (int)min(s.low - low, n);
-            col_high[nt][i] = (int)max(s.high - low, (int64_t)-1);
-        }
-
-    const uint32_t rank = !SHARED && a.cluster > 1 ? cluster_rank() : 0;
-    if (!SHARED) {
-        const uint32_t tiles = (uint32_t)((n + 15) / 16), share = tiles / a.cluster, extra = tiles - share * a.cluster;
-        first_tile = share * rank + min(rank, extra), last_tile = first_tile + share + (rank < extra);
-    }
-    const int begin = (int)first_tile, end = min((int)last_tile, (int)((n + 15) / 16));
-    const int64_t cell0 = (int64_t)head * a.max_slots + low;
-
-    float o[kBlocks][NT][4] = {}, o128[NT][4] = {};         // o128: 128 times the sum of the weights, in the codes' unit
-    // running maximum, sum, factor on weight * scale, and the largest weight * scale when it was set;
-    // the factor starts so large that the first weight * scale that is not zero sets it
-    float m[NT][2], l[NT][2] = {}, f[NT][2], big[NT][2] = {};
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, f[nt][0] = f[nt][1] = 0x1p126f;
-
-    const int dim = EXACT ? D : a.dim;
-    // A warp's tiles come through a ring in shared memory, each operand of a tile in D / 32 copies of 512
-    // consecutive bytes.  Past the last slot the last one is copied again, and past the last chunk of a
-    // row that one: whatever lies in the cache there (a NaN, say) does not reach a product.
-    constexpr int kRowChunks = D / 16, kRowsPerCopy = 32 / kRowChunks, kCopies = 16 / kRowsPerCopy;
-    const int copy_row = lane / kRowChunks, copy_chunk_at = EXACT ? lane % kRowChunks * 16 : min(lane % kRowChunks * 16, dim - 16);
-    const uint8_t *const key_base = a.k_codes + cell0 * dim + copy_chunk_at, *const value_base = a.v_codes + cell0 * dim + copy_chunk_at;
-    uint8_t *const ring = reinterpret_cast<uint8_t *>(shared) + warp * (kStages * kStageBytes);
-    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
-    const float *const scale_base = (c < 2 ? a.k_scales : a.v_scales) + cell0;      // scales of rows r and r + 8, for all lanes of r
-    auto fetch = [&](int tile, uint32_t stage) {
-        const int s0 = tile * 16, left = count - 1 - s0;
-        const uint8_t *const kp = key_base + (int64_t)s0 * dim, *const vp = value_base + (int64_t)s0 * dim;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(stage + 32 * D + lane * 4),
-                     "l"(scale_base + s0 + min(r + 8 * (c & 1), left))
-                     : "memory");
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-            const int row = i * kRowsPerCopy + copy_row, from = (left >= 15 ? row : min(row, left)) * dim;
-            const uint32_t to = stage + chunk_place<D>(row, lane % kRowChunks);
-            copy_chunk(to, kp + from);
-            copy_chunk(to + 16 * D, vp + from);
-        }
-    };
-    // which warp takes the first tile differs from CTA to CTA, so that no scheduler gets all the odd ones
-    const int turn_of = (warp + (int)blockIdx.x) & (kAttWarps - 1);
-    int ahead = begin + turn_of;
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-        if (ahead < end) fetch(ahead, ring_at + i * kStageBytes);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ahead += kAttWarps;
-    }
     int at_stage = 0;
     for (int tile = begin + turn_of; tile < end; tile += kAttWarps) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -815,56 +826,63 @@ template <int D, int NT> constexpr int kAttCtas = D == 128 ? 4 / NT : D == 64 ? 
 template <int D, int NT, int FMT, bool EXACT, typename T>
 __global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attention_kernel(AttentionArgs a)
 {
-    attend<D, NT, FMT, EXACT, false, T>(a, blockIdx.x / a.cluster, 0, 0, nullptr);
+    const uint32_t unit = blockIdx.x / a.cluster, b = unit / a.row_groups / a.kv_heads;
+    attend<D, NT, FMT, EXACT, false, T>(a, unit, length_of(a, b), start_of(a, b), 0, 0, nullptr);
 }
 
 template <int D, int NT, int FMT, bool EXACT, typename T>
 __global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attention_shared_kernel(AttentionArgs a)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");     // the joining kernel may take its places
-    const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, gridDim.x);
+    const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, a.batch * heads, gridDim.x);
     if ((uint64_t)share * blockIdx.x >= total) return;
     uint32_t at = share * blockIdx.x;
     const uint32_t end = min(at + share, total);
-    Sequence s = find_sequence<false>(a, at);
+    Sequence s = find_sequence(a, at);
+    int64_t length = length_of(a, s.index), start = start_of(a, s.index);
     bool front = true;
     while (at < end && s.tiles) {
         const uint32_t inside = at - s.before * heads, unit = inside / s.tiles, first = inside - unit * s.tiles;
-        const uint32_t last = min(s.tiles, first + (end - at));
-        float *ws = first == 0 && last == s.tiles ? nullptr
-                  : a.workspace + ((int64_t)blockIdx.x * 2 + !front) * (NT * 8 * (D + 2));
-        attend<D, NT, FMT, EXACT, true, T>(a, s.index * heads + unit, first, last, ws);
+        const uint32_t last = min(s.tiles, first + (end - at)), slot = blockIdx.x * 2 + !front;
+        const bool whole = first == 0 && last == s.tiles;
+        if (threadIdx.x == 0) {
+            // where the results are: nowhere but in `out`, or in the workspace from `slot` up to some CTA's
+            uint32_t *const cut = a.cuts + 2 * (s.index * heads + unit);
+            if (first == 0) cut[0] = whole ? kNotCut : slot;
+            if (last == s.tiles) cut[1] = blockIdx.x;
+        }
+        attend<D, NT, FMT, EXACT, true, T>(a, s.index * heads + unit, length, start, first, last,
+                                           whole ? nullptr : a.workspace + (int64_t)slot * (NT * 8 * (D + 2)));
         at += last - first;
         front = false;
         if (at < end && unit + 1 == heads && last == s.tiles) {
             s.before += s.tiles;
             do s.tiles = tiles_of(a, ++s.index); while (s.tiles == 0 && s.index < a.batch);
+            if (s.tiles) length = length_of(a, s.index), start = start_of(a, s.index);
         }
     }
 }
 
 // Joins the shares of a sequence that was cut, and writes the zeros of one that has no slots: one CTA
-// per query row, its threads in kJoinWays ways that take every so-manieth share.
-constexpr int kJoinWays = 4;
-template <int D, int NT, typename T> __global__ void __launch_bounds__(D * kJoinWays) kv_attention_join_kernel(AttentionArgs a, uint32_t ctas)
+// per query row, its threads in WAYS ways that take every WAYS-th share.
+template <int D, int NT, int WAYS, typename T> __global__ void __launch_bounds__(D * WAYS) kv_attention_join_kernel(AttentionArgs a)
 {
     constexpr int kRows = NT * 8, kSlot = kRows * (D + 2);
-    __shared__ float sums[kJoinWays][D], totals[kJoinWays], peaks[kJoinWays];
+    __shared__ float sums[WAYS][D], totals[WAYS], peaks[WAYS];
     const uint32_t rows = a.group * a.queries, at = blockIdx.x % rows, head = blockIdx.x / rows, b = head / a.kv_heads;
-    const uint32_t heads = a.kv_heads * a.row_groups, total = all_tiles(a) * heads, share = share_of(total, ctas);
-    const Sequence s = find_sequence<true>(a, b);
-    const uint32_t from = s.before * heads + (head % a.kv_heads * a.row_groups + at / kRows) * s.tiles;
-    const uint32_t j0 = from / share, j1 = s.tiles ? (from + s.tiles - 1) / share : j0;
+    const uint32_t tiles = tiles_of(a, b);
     asm volatile("griddepcontrol.wait;" ::: "memory");                  // the shares are written
-    if (s.tiles && j0 == j1) return;                                    // whole: written where it was computed
+    const uint32_t *const cut = a.cuts + 2 * (head * a.row_groups + at / kRows);
+    const uint32_t from = cut[0], last = cut[1];
+    if (tiles && from == kNotCut) return;                               // whole: written where it was computed
     const int row = (int)(at % kRows), d = threadIdx.x % D, way = threadIdx.x / D;
     float peak = -INFINITY, sum = 0.0f, l = 0.0f;
-    if (s.tiles) {
-        // the first share of the sequence may be the second of its CTA, all others are their CTA's first
-        auto part = [&](uint32_t j) { return a.workspace + ((int64_t)j * 2 + (j == j0 && j0 * share != from)) * kSlot; };
+    if (tiles) {
+        // the first share may be the second of its CTA, all others are their CTA's first
+        const uint32_t j0 = from / 2;
 #pragma unroll 4
-        for (uint32_t j = j0 + way; j <= j1; j += kJoinWays) {
-            const float *const x = part(j);
+        for (uint32_t j = j0 + way; j <= last; j += WAYS) {
+            const float *const x = a.workspace + (int64_t)(j == j0 ? from : j * 2) * kSlot;
             const float m = x[kRows * D + row], y = x[row * D + d], z = x[kRows * D + kRows + row];
             const float now = fmaxf(peak, m), old = peak == -INFINITY ? 0.0f : exp2_approx(peak - now);
             const float turn = m == -INFINITY ? 1.0f : exp2_approx(m - now);
@@ -873,19 +891,22 @@ template <int D, int NT, typename T> __global__ void __launch_bounds__(D * kJoin
             peak = now;
         }
     }
-    sums[way][d] = sum;
-    if (d == 0) totals[way] = l, peaks[way] = peak;
-    __syncthreads();
-    if (way || d >= a.dim) return;
+    if (WAYS > 1) {
+        sums[way][d] = sum;
+        if (d == 0) totals[way] = l, peaks[way] = peak;
+        __syncthreads();
+        if (way) return;
 #pragma unroll
-    for (int k = 1; k < kJoinWays; ++k) peak = fmaxf(peak, peaks[k]);
-    sum = l = 0.0f;
+        for (int k = 1; k < WAYS; ++k) peak = fmaxf(peak, peaks[k]);
+        sum = l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < kJoinWays; ++k) {
-        const float turn = peaks[k] == -INFINITY ? 1.0f : exp2_approx(peaks[k] - peak);
-        l += turn * totals[k];
-        sum += turn * sums[k][d];
+        for (int k = 0; k < WAYS; ++k) {
+            const float turn = peaks[k] == -INFINITY ? 1.0f : exp2_approx(peaks[k] - peak);
+            l += turn * totals[k];
+            sum += turn * sums[k][d];
+        }
     }
+    if (d >= a.dim) return;
     const uint32_t query = at / a.group, hq = head % a.kv_heads * a.group + (at - query * a.group);
     ((T *)a.out)[(((int64_t)b * a.queries + query) * (a.kv_heads * a.group) + hq) * a.dim + d] =
         df11_from_float<T>(l == 0.0f ? 0.0f : sum / l);
@@ -895,7 +916,7 @@ template <int D, int NT, typename T> __global__ void __launch_bounds__(D * kJoin
 struct Division {
     int width, tiles_n;         // padded head_dim, row tiles of 8
     int cluster;                // CTAs per unit; 0: the work is shared out
-    int64_t row_groups, units, ctas, workspace;
+    int64_t row_groups, units, ctas, cuts, workspace;
 };
 
 constexpr int kSms = 148;
@@ -909,7 +930,7 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
     d.tiles_n = rows > 8 && d.width < 256 ? 2 : 1;
     d.row_groups = (rows + d.tiles_n * 8 - 1) / (d.tiles_n * 8);
     d.units = batch * kv_heads * d.row_groups;
-    d.workspace = 0;
+    d.cuts = d.workspace = 0;
     const int64_t span = window > 0 && (int64_t)window + queries < max_slots ? window + queries : max_slots;
     const int64_t tiles = (span + 15) / 16;
     const int per_sm = d.width == 256 ? kAttCtas<256, 1> : d.width == 128 ? (d.tiles_n == 1 ? kAttCtas<128, 1> : kAttCtas<128, 2>)
@@ -917,7 +938,8 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
     if ((double)d.units * (double)tiles * d.width * 32 > kShareBytes && (double)d.units * (double)tiles < 2e9) {
         d.cluster = 0;
         d.ctas = kSms * per_sm;
-        d.workspace = d.ctas * 2 * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float);
+        d.cuts = (d.units * 2 * (int64_t)sizeof(uint32_t) + 15) / 16 * 16;
+        d.workspace = d.cuts + d.ctas * 2 * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float);
         return d;
     }
     const int64_t most = (tiles + 2 * kAttWarps - 1) / (2 * kAttWarps);                         // two tiles per warp
@@ -960,17 +982,21 @@ cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int devi
     const cudaError_t e = launch_wide(kv_attention_shared_kernel<D, NT, FMT, EXACT, T>, (unsigned)d.ctas, kAttWarps * 32, kShared, 1,
                                       device, stream, a);
     if (e != cudaSuccess) return e;
-    // the joining kernel is launched while the first still runs and waits for its end on the device
+    // The joining kernel is launched while the first still runs and waits for its end on the device.  Where many
+    // CTAs meet in a sequence, several threads share its results; otherwise small CTAs all fit at once.
+    constexpr int kWays = 1024 / D;
+    const bool many = d.ctas > 8 * d.units;
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3((unsigned)(d.units / d.row_groups * ((int64_t)a.group * a.queries)));
-    config.blockDim = dim3(D * kJoinWays);
+    config.blockDim = dim3(many ? D * kWays : D);
     config.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kv_attention_join_kernel<D, NT, T>, a, (uint32_t)d.ctas);
+    return many ? cudaLaunchKernelEx(&config, kv_attention_join_kernel<D, NT, kWays, T>, a)
+                : cudaLaunchKernelEx(&config, kv_attention_join_kernel<D, NT, 1, T>, a);
 }
 
 template <typename T> cudaError_t launch_attention(const AttentionArgs &a, const Division &d, int format, int device, cudaStream_t stream)
@@ -1119,7 +1145,7 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     a.k_scales = (const float *)k_scales, a.v_scales = (const float *)v_scales;
     a.lengths = (const int64_t *)lengths, a.length_per = n_lengths > 1;
     a.first = (const int64_t *)first, a.first_per = n_first > 1;
-    a.out = out, a.workspace = (float *)workspace;
+    a.out = out, a.cuts = (uint32_t *)workspace, a.workspace = (float *)((uint8_t *)workspace + d.cuts);
     a.kv_heads = (uint32_t)kv_heads, a.group = (uint32_t)(heads / kv_heads), a.dim = head_dim, a.window = window;
     a.batch = (uint32_t)batch, a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster;
     a.queries = (uint32_t)queries, a.max_slots = max_slots, a.scale = scale;
