@@ -97,52 +97,56 @@ template <int FMT> __device__ __forceinline__ uint32_t codes_of(const float (&x)
     return y;
 }
 
-// One block: rows of one sequence (blockIdx.y, and every gridDim.y-th after it); the value rows follow the
-// key rows.
+// The codes and the scale of one row, of which this thread has 16 numbers.
+template <int LANES, int FMT, typename T>
+__device__ __forceinline__ void quantise_row(const uint4 (&raw)[2], bool store, bool lead, uint8_t *to, float *scale)
+{
+    // magnitudes order like their bits, a NaN above an infinity
+    uint32_t bits = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) bits = __vmaxu2(bits, reinterpret_cast<const uint32_t *>(raw)[w] & 0x7FFF7FFFu);
+#pragma unroll
+    for (int d = LANES / 2; d; d >>= 1) bits = __vmaxu2(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+    if (!store) return;
+    bits = max(bits & 0xFFFFu, bits >> 16);
+    const bool finite = bits < kInfBits<T>, zero = bits == 0 || !finite;
+    const uint16_t top_bits = (uint16_t)bits;
+    const float most = FMT == DF11_KV_INT8 ? 127.0f : 448.0f, top = df11_to_float(*reinterpret_cast<const T *>(&top_bits));
+    // a power of two that keeps x * most away from overflow and x away from the subnormals
+    const float shift = top > 1e30f ? 0x1p-40f : top < 1e-30f ? 0x1p40f : 1.0f;
+    const float over = zero ? 1.0f : top * shift, up = shift * most, factor = up * __frcp_rn(over);
+    uint32_t codes[4];
+    const T *const x = reinterpret_cast<const T *>(raw);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float four[4] = {df11_to_float(x[4 * w]), df11_to_float(x[4 * w + 1]), df11_to_float(x[4 * w + 2]), df11_to_float(x[4 * w + 3])};
+        codes[w] = zero ? 0 : codes_of<FMT>(four, up, over, factor, shift != 1.0f);
+    }
+    *reinterpret_cast<uint4 *>(to) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+    if (lead) *scale = finite ? __fdiv_rn(top, most) : __int_as_float(0x7fc00000);
+}
+
+// One block: rows of one sequence (blockIdx.y, and every gridDim.y-th after it), keys and values; what
+// is loaded does not wait for the position.
 template <int LANES, int FMT, typename T> __global__ void __launch_bounds__(256) kv_append_kernel(AppendArgs a)
 {
     constexpr int kRows = 256 / LANES;
     const uint32_t per = a.heads * a.tokens, r = blockIdx.x * kRows + threadIdx.x / LANES;
     const int part = threadIdx.x % LANES * 16;
-    const bool value = r >= per, some = r < 2 * per;
-    const uint32_t within = some ? (value ? r - per : r) : 0, t = within / a.heads, h = within - t * a.heads;
-    const bool mine = some && part < a.dim;
+    const bool mine = r < per && part < a.dim;
+    const uint32_t within = mine ? r : 0, t = within / a.heads, h = within - t * a.heads;
     for (uint32_t b = blockIdx.y; b < a.batch; b += gridDim.y) {
+        uint4 key[2] = {}, value[2] = {};
+        if (mine) {
+            load16((const T *)a.k + b * a.ks.b + h * a.ks.h + t * a.ks.t + part, a.aligned, key);
+            load16((const T *)a.v + b * a.vs.b + h * a.vs.h + t * a.vs.t + part, a.aligned, value);
+        }
         const int64_t position = a.positions[a.per_sequence ? b : 0];
-        const bool there = position >= -(int64_t)t && position < a.max_slots - (int64_t)t;
-        uint4 raw[2] = {};
-        if (mine && there) {
-            const Strides s = value ? a.vs : a.ks;
-            load16((const T *)(value ? a.v : a.k) + b * s.b + h * s.h + t * s.t + part, a.aligned, raw);
-        }
-        // magnitudes order like their bits, a NaN above an infinity
-        uint32_t bits = 0;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) bits = __vmaxu2(bits, reinterpret_cast<const uint32_t *>(raw)[w] & 0x7FFF7FFFu);
-#pragma unroll
-        for (int d = LANES / 2; d; d >>= 1) bits = __vmaxu2(bits, __shfl_xor_sync(0xffffffffu, bits, d));
-        bits = max(bits & 0xFFFFu, bits >> 16);
-        if (!mine) continue;
-        if (!there) {
-            if (part == 0 && a.status) atomicOr(a.status, DF11_STATUS_BAD_POSITIONS);
-            continue;
-        }
-        const bool finite = bits < kInfBits<T>, zero = bits == 0 || !finite;
-        const uint16_t top_bits = (uint16_t)bits;
-        const float most = FMT == DF11_KV_INT8 ? 127.0f : 448.0f, top = df11_to_float(*reinterpret_cast<const T *>(&top_bits));
-        // a power of two that keeps x * most away from overflow and x away from the subnormals
-        const float shift = top > 1e30f ? 0x1p-40f : top < 1e-30f ? 0x1p40f : 1.0f;
-        const float over = zero ? 1.0f : top * shift, up = shift * most, factor = up * __frcp_rn(over);
-        uint32_t codes[4];
-        const T *const x = reinterpret_cast<const T *>(raw);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float four[4] = {df11_to_float(x[4 * w]), df11_to_float(x[4 * w + 1]), df11_to_float(x[4 * w + 2]), df11_to_float(x[4 * w + 3])};
-            codes[w] = zero ? 0 : codes_of<FMT>(four, up, over, factor, shift != 1.0f);
-        }
-        const int64_t cell = ((int64_t)b * a.heads + h) * a.max_slots + position + t;
-        *reinterpret_cast<uint4 *>((value ? a.v_codes : a.k_codes) + cell * a.dim + part) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-        if (part == 0) (value ? a.v_scales : a.k_scales)[cell] = finite ? __fdiv_rn(top, most) : __int_as_float(0x7fc00000);
+        const bool there = position >= -(int64_t)t && position < a.max_slots - (int64_t)t, store = mine && there;
+        const int64_t cell = there ? ((int64_t)b * a.heads + h) * a.max_slots + position + t : 0;
+        if (mine && !there && part == 0 && a.status) atomicOr(a.status, DF11_STATUS_BAD_POSITIONS);
+        quantise_row<LANES, FMT, T>(key, store, part == 0, a.k_codes + cell * a.dim + part, a.k_scales + cell);
+        quantise_row<LANES, FMT, T>(value, store, part == 0, a.v_codes + cell * a.dim + part, a.v_scales + cell);
     }
 }
 
@@ -194,7 +198,7 @@ template <int FMT, typename T> __global__ void __launch_bounds__(256) kv_read_ke
 
 template <int LANES, typename T> void launch_append(const AppendArgs &a, int format, cudaStream_t stream)
 {
-    const dim3 grid((unsigned)(((uint64_t)2 * a.heads * a.tokens + 256 / LANES - 1) / (256 / LANES)), a.batch < 65535 ? a.batch : 65535);
+    const dim3 grid((unsigned)(((uint64_t)a.heads * a.tokens + 256 / LANES - 1) / (256 / LANES)), a.batch < 65535 ? a.batch : 65535);
     if (format == DF11_KV_INT8) kv_append_kernel<LANES, DF11_KV_INT8, T><<<grid, 256, 0, stream>>>(a);
     else kv_append_kernel<LANES, DF11_KV_E4M3, T><<<grid, 256, 0, stream>>>(a);
 }

@@ -385,7 +385,8 @@ int df11_encode_device_pack(const void *exponents, int64_t n_elements, const voi
  *     DF11_KV_INT8   scale = a / 127, code = x * 127 / a to the nearest integer (ties to even)
  *     DF11_KV_E4M3   scale = a / 448, code = x * 448 / a to the nearest e4m3 (ties to even)
  * and stands for code * scale.  The code is the one of the exact quotient.  A row of zeros has
- * scale 0; a row with an infinity or a NaN has scale NaN and codes 0 (it stands for NaNs).
+ * scale 0; a row with an infinity or a NaN has scale NaN and codes 0 (it stands for NaNs).  Codes
+ * are never NaN; what stands for an e4m3 NaN in a cache written by others is not kept apart.
  */
 #define DF11_TYPE_BF16 0
 #define DF11_TYPE_FP16 1

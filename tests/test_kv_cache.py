@@ -435,6 +435,27 @@ def test_step_in_a_graph_beside_another_stream():
 
 
 @gpu
+def test_offsets_beyond_32_bits():
+    """A cache of more than 2^32 codes: its last slots are written, read and attended to like any others."""
+    slots, dim, n = (1 << 26) + 40, 64, 40
+    cache = new_cache(1, 1, slots, dim, "int8")
+    x, y = (random_rows((1, 1, n, dim), torch.bfloat16, s) for s in (50, 51))
+    ops.kv_append(x.to(DEV), y.to(DEV), *cache, torch.tensor([slots - n], device=DEV))
+    for got, rows in zip(ops.kv_read(*cache, slots - n, n), (x, y)):
+        want, scale = reference_rows(rows, "int8")
+        assert torch.equal(got.cpu(), (want.float() * scale[..., None]).to(torch.bfloat16))
+    assert not cache[0][:, :, :1000].any() and not cache[1][:, :, :slots - n].any()
+    tail = tuple(t[:, :, slots - n:].clone() for t in cache)
+    q = query(1, 4, 1, dim, torch.bfloat16, 52)
+    want, bound = reference_attention(q, tail, [n], [0], dim ** -0.5, 0)
+    for window, first in ((0, slots - n), (n, 0)):
+        got = ops.kv_attention(q, *cache, torch.tensor([slots], device=DEV), first=torch.tensor([first], device=DEV), window=window)
+        assert ((got.cpu().double() - want).abs() <= bound + want.abs() * 2.0 ** -8).all()
+    del cache, tail
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_nothing_to_do():
     cache = filled_cache(2, 1, 8, 64, "int8", seed=23)
     none = torch.empty(2, 1, 0, 64, dtype=torch.bfloat16, device=DEV)
