@@ -28,6 +28,8 @@
 // cluster barriers, for many the fp64 units (nine operations per token at half a clock per warp each).
 #include <math.h>
 
+#include <type_traits>
+
 #include "df11_launch.h"
 
 namespace {
@@ -330,6 +332,7 @@ __device__ __forceinline__ u64 draw_of(double u, u64 total)
 // ---------------------------------------------------------------------------------------------
 // The row's tokens in groups of 8 that start on a 16-byte (or, of floats, a 32-byte) boundary.
 template <typename T> struct Tokens {
+    static constexpr uint32_t kInfPair = std::is_same<T, __half>::value ? 0xFC00FC00u : 0xFF80FF80u;
     const T *row;
     uint32_t vocab;
     int lead;                                 // tokens that the first group lacks
@@ -339,20 +342,63 @@ template <typename T> struct Tokens {
         lead = (int)(reinterpret_cast<uintptr_t>(r) / sizeof(T) % 8);
         groups = (v + lead + 7) / 8;
     }
-    // The logits of group g; -inf for a NaN and where there is no token.  Token j of it has the index 8 g - lead + j.
-    __device__ __forceinline__ void logits(uint32_t g, float (&z)[8]) const
+    struct Raw {
+        uint4 words[sizeof(T) / 2];
+    };
+    // Group g as it lies in memory; -inf where there is no token.  Token j of it has the index 8 g - lead + j.
+    __device__ __forceinline__ Raw load(uint32_t g) const
     {
+        Raw raw;
         const int64_t first = (int64_t)g * 8 - lead;
         if (first >= 0 && first + 8 <= vocab) {
-            uint4 raw[sizeof(T) / 2];
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(row + first) + i);
-            const T *x = reinterpret_cast<const T *>(raw);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = fmaxf(df11_to_float(x[j]), -INFINITY);
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw.words[i] = __ldg(reinterpret_cast<const uint4 *>(row + first) + i);
         } else {
+            constexpr uint32_t kNone = sizeof(T) == 4 ? 0xFF800000u : kInfPair;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = first + j >= 0 && first + j < vocab ? fmaxf(df11_to_float(row[first + j]), -INFINITY) : -INFINITY;
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw.words[i] = make_uint4(kNone, kNone, kNone, kNone);
+            T *const x = reinterpret_cast<T *>(raw.words);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (first + j >= 0 && first + j < vocab) x[j] = row[first + j];
+        }
+        return raw;
+    }
+    // Its logits; -inf for a NaN.
+    __device__ __forceinline__ static void unpack(const Raw &raw, float (&z)[8])
+    {
+        const T *const x = reinterpret_cast<const T *>(raw.words);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = fmaxf(df11_to_float(x[j]), -INFINITY);
+    }
+    // Calls f(g, logits) for g = first, first + step, ... below `end`, with four groups on their way at once.
+    template <typename F> __device__ __forceinline__ void each4(uint32_t first, uint32_t end, uint32_t step, F f) const
+    {
+        for (uint32_t g = first; g < end; g += 4 * step) {
+            Raw raw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (g + i * step < end) raw[i] = load(g + i * step);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (g + i * step >= end) break;
+                float z[8];
+                unpack(raw[i], z);
+                f(g + i * step, z);
+            }
+        }
+    }
+    // Calls f(g, logits) for g = first, first + step, ... below `end`; the next group is on its way meanwhile.
+    template <typename F> __device__ __forceinline__ void each(uint32_t first, uint32_t end, uint32_t step, F f) const
+    {
+        if (first >= end) return;
+        Raw next = load(first);
+        for (uint32_t g = first; g < end; g += step) {
+            const Raw now = next;
+            if (g + step < end) next = load(g + step);
+            float z[8];
+            unpack(now, z);
+            f(g, z);
         }
     }
     __device__ __forceinline__ float at(int64_t i) const { return fmaxf(df11_to_float(row[i]), -INFINITY); }
@@ -594,16 +640,13 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     // the largest and the smallest logit
     const bool greedy = !(row.t > 0.0), few = !greedy && row.k > 0 && row.k <= kFewTokens;
     float top = -INFINITY, bottom = INFINITY;
-#pragma unroll 4
-    for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-        float z[8];
-        tokens.logits(g, z);
+    tokens.each4(g0 + tid, g1, kThreads, [&](uint32_t, const float (&z)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             top = fmaxf(top, z[j]);
             bottom = fminf(bottom, z[j] > -INFINITY ? z[j] : INFINITY);
         }
-    }
+    });
     if (tid < kRoots) s.roots[tid] = exp2((double)tid / kRoots);
     if (tid == 0) s.mine.bound = -INFINITY, s.list_n = 0, s.found = kAny;
     {
@@ -656,14 +699,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     Shared &head = *(size > 1 ? remote(&s, 0) : &s);
     if (greedy) {
         uint32_t index = kAny;
-#pragma unroll 4
-        for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-            float z[8];
-            tokens.logits(g, z);
+        tokens.each4(g0 + tid, g1, kThreads, [&](uint32_t g, const float (&z)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (z[j] == best) index = min(index, g * 8 - tokens.lead + j);
-        }
+        });
         index = __reduce_min_sync(0xffffffffu, index);
         if (lane == 0 && index != kAny) atomicMin(&head.found, index);
         cluster_sync(size);
@@ -700,14 +740,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     };
     if (few) {
         bound = fmaxf(bound, lowest);
-#pragma unroll 4
-        for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-            float z[8];
-            tokens.logits(g, z);
+        tokens.each4(g0 + tid, g1, kThreads, [&](uint32_t g, const float (&z)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (z[j] >= bound) list_token(z[j], g * 8 - tokens.lead + j);
-        }
+        });
         cluster_sync(size);
         const uint32_t n = rank == 0 ? collect() : 0;
         if (size > 1) cluster_sync(size);
@@ -716,6 +753,28 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
         else sample_slowly(tokens, row, lowest, weigh, a.out + at);
         return;
     }
+
+    // Calls f(g, logits, part) for all groups, a block per warp; what f adds to `part` becomes the block's sum.
+    auto each_block = [&](auto f) {
+        if ((uint32_t)warp >= blocks) return;
+        const uint32_t last_of = (1u << wide) - 1, steps = (blocks - warp + kWarps - 1) / kWarps << wide;
+        auto group_of = [&](uint32_t q) { return g0 + (warp + (q >> wide) * kWarps) * block_groups + (q & last_of) * 32 + lane; };
+        u64 part = 0;
+        for (uint32_t q = 0; q < steps; ++q) {
+            const uint32_t g = group_of(q);
+            if (g < g1) {
+                float z[8];
+                tokens.unpack(tokens.load(g), z);
+                f(g, z, part);
+            }
+            if ((q & last_of) == last_of) {
+#pragma unroll
+                for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+                if (lane == 0) s.blocks[warp + (q >> wide) * kWarps] = part;
+                part = 0;
+            }
+        }
+    };
 
     float kept_logit = lowest;                                          // the filters' border so far
     uint32_t kept_index = kAny;
@@ -732,14 +791,11 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
         auto bin_of = [&](float z) { return (int)(__float_as_uint(place_of(fminf(z, from))) & (kBins - 1)); };
         for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
         __syncthreads();
-#pragma unroll 2
-        for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-            float z[8];
-            tokens.logits(g, z);
+        tokens.each(g0 + tid, g1, kThreads, [&](uint32_t, const float (&z)[8]) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (z[j] >= lowest) atomicAdd(&s.count[bin_of(z[j])], 1u);
-        }
+        });
         cluster_sync(size);
         if (size > 1) {
             for (int i = (int)rank * (kBins / (int)size) + tid; i < ((int)rank + 1) * (kBins / (int)size); i += kThreads) {
@@ -808,17 +864,14 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             const int bin = s.bin_k;
             // what top-k keeps, as a whole or the interval of its border
             const bool all = s.above_k + count[bin] <= (uint32_t)kList;
-#pragma unroll 2
-            for (uint32_t g = g0 + tid; g < g1; g += kThreads) {
-                float z[8];
-                tokens.logits(g, z);
+            tokens.each(g0 + tid, g1, kThreads, [&](uint32_t g, const float (&z)[8]) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     if (z[j] >= lowest) {
                         const int b = bin_of(z[j]);
                         if (b == bin || (all && b < bin)) list_token(z[j], g * 8 - tokens.lead + j);
                     }
-            }
+            });
             cluster_sync(size);
             if (rank == 0) {
                 const uint32_t n = collect();
@@ -859,13 +912,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             const float low = kMagic + s.bin_low, high = kMagic + s.bin_high;
             u64 mass_all = 0, mass_above = 0;
             auto add_up = [&](auto filtered, auto plain) {
-                for (uint32_t block = warp; block < blocks; block += kWarps) {
-                    u64 part = 0;
-                    for (int x = 0; x < 1 << wide; ++x) {
-                        const uint32_t g = g0 + block * block_groups + x * 32 + lane, index = g * 8 - tokens.lead;
-                        if (g >= g1) continue;
-                        float z[8];
-                        tokens.logits(g, z);
+                each_block([&](uint32_t g, const float (&z)[8], u64 &part) {
+                        const uint32_t index = g * 8 - tokens.lead;
                         uint32_t on_list = 0;
                         u64 above = 0;
 #pragma unroll
@@ -887,11 +935,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                             for (int j = 0; j < 8; ++j)
                                 if (on_list >> j & 1) list_token(z[j], index + j);
                         }
-                    }
-#pragma unroll
-                    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-                    if (lane == 0) s.blocks[block] = part;
-                }
+                });
             };
             if (!weigh.plain) add_up(Yes{}, No{});
             else if (by_rank || floor > 0.0) add_up(Yes{}, Yes{});
@@ -937,24 +981,14 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
     }
     if (!by_mass) {
         auto add_up = [&](auto filtered, auto plain) {
-            for (uint32_t block = warp; block < blocks; block += kWarps) {
-                u64 part = 0;
-                for (int x = 0; x < 1 << wide; ++x) {
-                    const uint32_t g = g0 + block * block_groups + x * 32 + lane;
-                    if (g >= g1) continue;
-                    float z[8];
-                    tokens.logits(g, z);
+            each_block([&](uint32_t g, const float (&z)[8], u64 &part) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
-                        part += weigh.biased(!filtered.value || (is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor) ? w : 0.0);
-                    }
-                    part -= 8 * weigh.kBias;
+                for (int j = 0; j < 8; ++j) {
+                    const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
+                    part += weigh.biased(!filtered.value || (is_kept(z[j], g * 8 - tokens.lead + j) && w >= floor) ? w : 0.0);
                 }
-#pragma unroll
-                for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-                if (lane == 0) s.blocks[block] = part;
-            }
+                part -= 8 * weigh.kBias;
+            });
         };
         if (!weigh.plain) add_up(Yes{}, No{});
         else if (by_rank || floor > 0.0) add_up(Yes{}, Yes{});
@@ -982,7 +1016,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             for (int x = 0; x < 1 << wide; ++x) {
                 const uint32_t g = g0 + s.found * block_groups + x * 32 + lane;
                 float z[8];
-                if (g < g1) tokens.logits(g, z);
+                if (g < g1) tokens.unpack(tokens.load(g), z);
                 u64 w[8];
                 sum = 0;
 #pragma unroll
