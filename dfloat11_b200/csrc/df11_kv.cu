@@ -23,7 +23,9 @@ struct Strides {
     int64_t b, h, t;
 };
 
-// Writing and reading move bytes and compute little: 3 bytes per number either way.  A group of LANES
+// Writing and reading move bytes and compute little: 3 bytes per number either way.  65536 rows of 128 keys and
+// values each (403 MB): written in 79 us (5.1 TB/s; some 9 instructions per number keep it from the copy rate), read
+// in 63 us (6.4 TB/s, the copy rate).  A group of LANES
 // threads (a power of two) holds a row in registers, 16 numbers per thread, so that a row's maximum is a few
 // shuffles and its codes leave as one 16-byte store per thread.
 // 16 numbers from an address that may have any alignment of the type.
@@ -236,11 +238,20 @@ template <typename T> void launch_append(const AppendArgs &a, int format, cudaSt
 // Sums, maxima and denominators are fp32.
 //
 // Small calls: the slots of a sequence are divided among a cluster of CTAs that join their results
-// through distributed shared memory, in one launch.  Large ones: the tiles of all sequences and heads are
+// through distributed shared memory, in one launch.  Long ones: the tiles of all sequences and heads are
 // cut into equal lengths, one per resident CTA, so that sequences of any lengths keep every SM busy
 // to the end; a second kernel joins, in a fixed order, what was cut.
+//
+// Why mma.sync: with 4 to 16 query rows the tensor pipe is 15 % busy; a tcgen05 tile would be filled to an
+// eighth and would want the widened operands written back to shared memory.  What bounds it: memory, with
+// the instructions that widen and weigh (about 300 per tile of 16 slots) close behind, and 3 us per stretch for
+// its start and end.  Measured in a graph of such calls: 131071 slots x 8 heads of 128 (277 MB) 55 us = 5.0 TB/s, of
+// which the loads alone take 50; 32 left-padded sequences of 2048-4096 slots (174 MB) 39 us = 4.4 TB/s.  Copies of
+// 512 consecutive bytes instead of the fragments' own 64-byte pieces: 78 -> 59 us for the former.
 constexpr int kAttWarps = 4;
-template <int D> constexpr int kAttStages = D == 64 ? 4 : 3;       // tiles of 16 slots under way per warp, one in use
+// Tiles of 16 slots under way per warp, one in use.  Heads of 128: four with three CTAs per SM against three with
+// four CTAs, 32 ragged sequences 39.4 and 40.2 us, 131071 slots 54.8 and 56.9 us.
+template <int D> constexpr int kAttStages = D == 256 ? 3 : 4;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void mma_16x8x16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -825,7 +836,7 @@ __device__ __forceinline__ void attend(const AttentionArgs &a, uint32_t unit, in
     if (SHARED) __syncthreads();                        // the next stretch fills the same memory
 }
 
-template <int D, int NT> constexpr int kAttCtas = D == 128 ? 4 / NT : D == 64 ? 5 - NT : 2;   // per SM, by registers and memory
+template <int D, int NT> constexpr int kAttCtas = D == 256 ? 2 : D == 128 ? 4 - NT : 5 - NT;     // per SM, by registers and memory
 
 template <int D, int NT, int FMT, bool EXACT, typename T>
 __global__ void __launch_bounds__(kAttWarps * 32, (kAttCtas<D, NT>)) kv_attention_kernel(AttentionArgs a)
@@ -924,7 +935,10 @@ struct Division {
 };
 
 constexpr int kSms = 148;
-constexpr double kShareBytes = 16e6;
+// Codes that a warp of a cluster may have to read at most.  Above it, sharing out pays for its second launch and the
+// joining: 8 key heads of 128, 8192 slots (64 KB per warp): cluster 12.7 us, shared out 15.7; 16384 slots: 19.2
+// and 17.5; 2 heads, 32768 slots: 32 and 24; 32 sequences of 1024 slots (32 KB): 16.2 and 21.9.
+constexpr int64_t kLongStretch = 96 << 10;
 
 Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries, int32_t head_dim, int64_t max_slots, int32_t window)
 {
@@ -939,18 +953,18 @@ Division divide(int64_t batch, int32_t heads, int32_t kv_heads, int64_t queries,
     const int64_t tiles = (span + 15) / 16;
     const int per_sm = d.width == 256 ? kAttCtas<256, 1> : d.width == 128 ? (d.tiles_n == 1 ? kAttCtas<128, 1> : kAttCtas<128, 2>)
                                                          : (d.tiles_n == 1 ? kAttCtas<64, 1> : kAttCtas<64, 2>);
-    if ((double)d.units * (double)tiles * d.width * 32 > kShareBytes && (double)d.units * (double)tiles < 2e9) {
-        d.cluster = 0;
-        d.ctas = kSms * per_sm;
-        d.cuts = (d.units * 2 * (int64_t)sizeof(uint32_t) + 15) / 16 * 16;
-        d.workspace = d.cuts + d.ctas * 2 * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float);
-        return d;
-    }
     const int64_t most = (tiles + 2 * kAttWarps - 1) / (2 * kAttWarps);                         // two tiles per warp
     int64_t want = d.units > 0 ? kSms * per_sm / d.units : 1;
     if (want > most) want = most;
     d.cluster = want >= 8 ? 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
     d.ctas = d.units * d.cluster;
+    const int64_t bytes_per_warp = (tiles + d.cluster * kAttWarps - 1) / (d.cluster * kAttWarps) * 32 * d.width;
+    if (bytes_per_warp > kLongStretch && (double)d.units * (double)tiles < 2e9) {
+        d.cluster = 0;
+        d.ctas = kSms * per_sm;
+        d.cuts = (d.units * 2 * (int64_t)sizeof(uint32_t) + 15) / 16 * 16;
+        d.workspace = d.cuts + d.ctas * 2 * d.tiles_n * 8 * (d.width + 2) * (int64_t)sizeof(float);
+    }
     return d;
 }
 

@@ -25,7 +25,9 @@
 //
 // A row is divided among a cluster of 1 to 8 CTAs, as many as leave every SM with work.  The row is
 // read two or three times, the first time from memory, then from the L2 cache.  Bound: for few rows the chain of
-// cluster barriers, for many the fp64 units (nine operations per token at half a clock per warp each).
+// barriers, for many the instructions (27 per token where weights are added up, 11 where tokens are counted).
+// Measured in a graph of such calls, rows of 151936 (one) and 128256 (256) BF16 logits: arg-max 6.3 and 30.5 us,
+// top-k of 20 with top-p 14.9 and 38.5, no filter 13.8 and 73, top-p 0.9 alone 38 and 157.
 #include <math.h>
 
 #include <type_traits>
@@ -40,7 +42,9 @@ constexpr int kBins = 4096;
 constexpr int kList = 2048;
 constexpr int kFew = 128;                     // numbers that are compared with one another
 constexpr int kBlocks = kThreads;             // block sums per CTA, at most
-constexpr int kFewTokens = 256;               // top-k up to here goes by the threads' largest
+// Top-k up to here goes by the threads' largest (one row of 151936, k = 20: 14.5 us); beyond, the bound lets through
+// more and more, and with k above the number of threads there is none: by counts (k = 500: 20.5 us).
+constexpr int kFewTokens = 256;
 constexpr uint32_t kLowestKey = 0x00800000u;  // key of the lowest finite float
 constexpr uint32_t kAny = 0xFFFFFFFFu;
 

@@ -263,7 +263,7 @@ def test_attention_window_and_padding(window, queries):
 
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("batch,heads,slots,queries", [(1, 1, 20011, 1), (1, 2, 9000, 3), (7, 3, 2500, 1), (40, 4, 700, 1), (3, 8, 5000, 1)])
+@pytest.mark.parametrize("batch,heads,slots,queries", [(1, 1, 20011, 1), (300, 2, 40, 1), (2, 4, 8000, 2), (1, 2, 9000, 3), (7, 3, 2500, 1), (40, 4, 700, 1), (3, 8, 5000, 1)])
 def test_attention_long(fmt, batch, heads, slots, queries):
     cache = filled_cache(batch, heads, slots, 64, fmt, seed=11)
     lengths = torch.tensor([slots - (b * 977) % slots for b in range(batch)], device=DEV)
@@ -273,21 +273,21 @@ def test_attention_long(fmt, batch, heads, slots, queries):
 @gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dim,group,queries,kv_heads,slots,lengths", [
-    (128, 4, 1, 4, 9000, [0, 8999, 1, 0, 0, 17, 300, 9000, 0]),         # one sequence among CTAs, many in one CTA
+    (128, 4, 1, 4, 13000, [0, 8999, 1, 0, 0, 17, 300, 13000, 0]),       # one sequence among CTAs, many in one CTA
     (128, 4, 1, 4, 40000, [39999]),
-    (128, 4, 1, 8, 8000, [0] * 3),                                      # nothing at all
-    (64, 2, 3, 4, 12000, [5, 2500, 0, 2, 4000, 33, 12000]),
+    (128, 4, 1, 8, 13000, [0] * 3),                                     # nothing at all
+    (64, 2, 3, 4, 25000, [5, 2500, 0, 2, 4000, 33, 25000]),
     (256, 5, 4, 2, 9000, [700, 3, 0, 1111]),                            # three row groups
-    (80, 16, 2, 2, 9000, [64, 1000, 0, 2]),
-    (128, 1, 1, 2, 600, [(37 * b) % 600 for b in range(75)]),           # more sequences than a warp has lanes
-    (96, 3, 1, 16, 300, [300 - b % 2 for b in range(70)]),
+    (80, 16, 2, 2, 13000, [64, 1000, 0, 2]),
+    (128, 1, 1, 2, 3300, [(37 * b) % 600 for b in range(75)]),           # more sequences than a warp has lanes
+    (96, 3, 1, 16, 1700, [300 - b % 2 for b in range(70)]),
 ])
-@pytest.mark.parametrize("window", [0, 333])
-def test_attention_shared_out(fmt, dim, group, queries, kv_heads, slots, lengths, window):
+@pytest.mark.parametrize("windowed", [False, True])
+def test_attention_shared_out(fmt, dim, group, queries, kv_heads, slots, lengths, windowed):
     """Caches so large that the tiles of all sequences are shared out evenly; lengths of any kind in them."""
-    batch = len(lengths)
+    batch, window = len(lengths), slots - 100 if windowed else 0
     shape = (batch, kv_heads, slots, dim)
-    need = _lib.lib.df11_kv_attention_workspace_bytes(batch, kv_heads * group, kv_heads, queries, dim, slots, 0)
+    need = _lib.lib.df11_kv_attention_workspace_bytes(batch, kv_heads * group, kv_heads, queries, dim, slots, window)
     assert need > 0, "this case is meant to take the shared-out kernel"
     cache = new_cache(*shape, fmt)
     g = torch.Generator(device=DEV).manual_seed(40)
