@@ -349,7 +349,7 @@ struct AttentionArgs {
     void *out;
     uint32_t *cuts;                     // shared out: per unit, the first result and the last CTA
     float *workspace;                   // and two results of rows * (D + 2) numbers per CTA
-    uint32_t batch, kv_heads, group, queries, row_groups, cluster;
+    uint32_t batch, kv_heads, group, queries, row_groups, cluster, ctas;
     int dim, window, q_aligned;
     int64_t max_slots;
     float scale;
@@ -436,7 +436,7 @@ __device__ __forceinline__ uint32_t cluster_rank()
 
 __device__ __forceinline__ void cluster_barrier()
 {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t remote_address(const float *local, uint32_t rank)
@@ -889,7 +889,7 @@ template <int D, int NT, int WAYS, typename T> __global__ void __launch_bounds__
     asm volatile("griddepcontrol.wait;" ::: "memory");                  // the shares are written
     const uint32_t *const cut = a.cuts + 2 * (head * a.row_groups + at / kRows);
     const uint32_t from = cut[0], last = cut[1];
-    if (tiles && from == kNotCut) return;                               // whole: written where it was computed
+    if (tiles && (from == kNotCut || from / 2 > last || last >= a.ctas)) return;    // whole: written where it was computed
     const int row = (int)(at % kRows), d = threadIdx.x % D, way = threadIdx.x / D;
     float peak = -INFINITY, sum = 0.0f, l = 0.0f;
     if (tiles) {
@@ -1165,7 +1165,7 @@ extern "C" int df11_kv_attention(const void *q, int64_t q_stride_b, int64_t q_st
     a.first = (const int64_t *)first, a.first_per = n_first > 1;
     a.out = out, a.cuts = (uint32_t *)workspace, a.workspace = (float *)((uint8_t *)workspace + d.cuts);
     a.kv_heads = (uint32_t)kv_heads, a.group = (uint32_t)(heads / kv_heads), a.dim = head_dim, a.window = window;
-    a.batch = (uint32_t)batch, a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster;
+    a.batch = (uint32_t)batch, a.row_groups = (uint32_t)d.row_groups, a.cluster = (uint32_t)d.cluster, a.ctas = (uint32_t)d.ctas;
     a.queries = (uint32_t)queries, a.max_slots = max_slots, a.scale = scale;
     const cudaError_t e = element_type == DF11_TYPE_BF16 ? launch_attention<__nv_bfloat16>(a, d, format, device, (cudaStream_t)stream)
                                                          : launch_attention<__half>(a, d, format, device, (cudaStream_t)stream);

@@ -171,7 +171,7 @@ extern __shared__ __align__(16) unsigned char raw_shared[];
 
 __device__ __forceinline__ void cluster_sync(uint32_t size)
 {
-    if (size > 1) asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+    if (size > 1) asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
     else __syncthreads();
 }
 

@@ -193,7 +193,7 @@ def for_model(config, max_slots: int, fmt: str = "int8", status: Optional[torch.
     """A ``transformers`` cache over a ``QuantizedKVCache`` for a decoder of this configuration.
 
     The codes are allocated with the first tokens, for their batch, heads (of a tensor-parallel shard: its own) and device;
-    ``.store`` is then the ``QuantizedKVCache``.  The model has to run with ``set_attn_implementation("df11_kv")``, for
+    ``.store`` is then the ``QuantizedKVCache``; all of the model's layers are on that device.  The model has to run with ``set_attn_implementation("df11_kv")``, for
     which ``GraphedGreedyDecoder(kv_format=...)`` cares.  ``status``: int32 word for ``STATUS_BAD_POSITIONS``."""
     if fmt not in FORMATS:
         raise ValueError(f"unknown cache format {fmt!r}: {', '.join(FORMATS)} are supported")
