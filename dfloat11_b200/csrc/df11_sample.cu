@@ -885,8 +885,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
                     draw_from_list((int)n, row, weigh, a.out + at);
                     if (tid == 0) s.verdict.fallback = 2;
                 } else {
-                    const u64 last = ~find_border((int)n, ByRank(), ByCount(),
-                                                  (u64)(limit - s.above_k));
+                    const u64 last = ~find_border((int)n, ByRank(), ByCount(), (u64)(limit - s.above_k));
                     if (tid == 0) s.verdict.logit = listed_logit(last), s.verdict.index = listed_index(last);
                 }
             }
@@ -917,28 +916,28 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 2) sample_kern
             u64 mass_all = 0, mass_above = 0;
             auto add_up = [&](auto filtered, auto plain) {
                 each_block([&](uint32_t g, const float (&z)[8], u64 &part) {
-                        const uint32_t index = g * 8 - tokens.lead;
-                        uint32_t on_list = 0;
-                        u64 above = 0;
+                    const uint32_t index = g * 8 - tokens.lead;
+                    uint32_t on_list = 0;
+                    u64 above = 0;
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const bool kept = !filtered.value || is_kept(z[j], index + j);
-                            const float place = place_of(plain.value ? z[j] : fminf(z[j], from));
-                            const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
-                            const u64 all = weigh.biased(kept ? w : 0.0);
-                            mass_all += all;
-                            above += place < low ? all : weigh.kBias;
-                            if (filtered.value) part += place < low && w >= floor ? all : weigh.kBias;
-                            if (place >= low && place <= high && kept && z[j] >= lowest) on_list |= 1u << j;
-                        }
-                        mass_all -= 8 * weigh.kBias, above -= 8 * weigh.kBias;
-                        mass_above += above;
-                        part += filtered.value ? 0 - 8 * weigh.kBias : above;
-                        if (on_list) {
+                    for (int j = 0; j < 8; ++j) {
+                        const bool kept = !filtered.value || is_kept(z[j], index + j);
+                        const float place = place_of(plain.value ? z[j] : fminf(z[j], from));
+                        const double w = plain.value ? weigh.fast(z[j]) : weigh.real(z[j]);
+                        const u64 all = weigh.biased(kept ? w : 0.0);
+                        mass_all += all;
+                        above += place < low ? all : weigh.kBias;
+                        if (filtered.value) part += place < low && w >= floor ? all : weigh.kBias;
+                        if (place >= low && place <= high && kept && z[j] >= lowest) on_list |= 1u << j;
+                    }
+                    mass_all -= 8 * weigh.kBias, above -= 8 * weigh.kBias;
+                    mass_above += above;
+                    part += filtered.value ? 0 - 8 * weigh.kBias : above;
+                    if (on_list) {
 #pragma unroll
-                            for (int j = 0; j < 8; ++j)
-                                if (on_list >> j & 1) list_token(z[j], index + j);
-                        }
+                        for (int j = 0; j < 8; ++j)
+                            if (on_list >> j & 1) list_token(z[j], index + j);
+                    }
                 });
             };
             if (!weigh.plain) add_up(Yes{}, No{});
